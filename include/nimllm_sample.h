@@ -340,6 +340,107 @@ NLS_API nls_status nls_lm_head_sample(nls_handle* h, const void* weights, int32_
                                       const double* uniforms, int64_t* out_ids, float* out_probs,
                                       uint32_t flags, void* stream);
 
+/* ---- 4-bit weights with group scales ---------------------------------------
+ * An output projection (or any weight matrix) whose weights are 4-bit values
+ * with one scale, and optionally one minimum, per group of consecutive
+ * columns of a row, and a sampler for the logits it writes. No counterpart in
+ * the reference, whose 4-bit types are ggml blocks (nls_lm_head): this is the
+ * form that round-to-nearest, error-compensating and activation-aware
+ * quantisers of half-precision checkpoints produce. Both entry points follow
+ * their definition in real arithmetic (not the reference's fp32 order). */
+
+/* element types of activations, scales and logits */
+#define NLS_DT_F32 0
+#define NLS_DT_F16 1
+#define NLS_DT_BF16 2
+
+/* A rows x cols weight matrix. Value q of (row r, column c) is the low nibble
+ * (c even) or high nibble (c odd) of byte c / 2 of row r. With group g =
+ * c / group, s = scales[g * s_ld + r] and m = mins[g * s_ld + r]:
+ *   w = s * (q - 8)   where mins is NULL,   w = s * q + m   otherwise.
+ * All pointers are device memory of the handle's device. A rank of a
+ * vocabulary split takes rows [lo, hi) of the same arrays by offsetting q by
+ * lo * q_ld and scales and mins by lo elements (lo a multiple of 8). */
+typedef struct nls_g4_weights {
+  const void* q;      /* 16-byte aligned */
+  const void* scales; /* 16-byte aligned; ceil(cols / group) lines of rows values, each with
+                         room for rows rounded up to 8 (what lies there is not used) */
+  const void* mins;   /* as scales, or NULL */
+  int64_t q_ld;       /* bytes from a row of q to the next: a multiple of 16, >= cols / 2 */
+  int64_t s_ld;       /* values from a group's line to the next: a multiple of 8, >= rows */
+  int32_t rows;
+  int32_t cols;       /* a multiple of 32 */
+  int32_t group;      /* 32, 64 or a multiple of 128; the last group may be short */
+  int32_t stype;      /* type of scales and mins: NLS_DT_* */
+} nls_g4_weights;
+
+/* y[b * ldy + r] = sum over c of w(r, c) * x[b * ldx + c] for b < nb.
+ *  x  nb rows of cols activations of type xtype, ldx >= cols values apart
+ *  y  nb rows of w->rows values of type ytype, ldy >= w->rows apart; what lies
+ *     behind a row's w->rows values is left as it was
+ * Products of a 4-bit value and an activation are exact (fp32 activations are
+ * taken as three bfloat16 parts); they are summed in fp32 per group, the
+ * groups' terms in fp32, and rounded once to ytype. fp32 and bfloat16
+ * activations are shifted by 2^-12 on the way, so that sums before the scales
+ * cannot overflow; what they lose lies below 2^-110. A batch row that holds an
+ * infinity or a NaN gets non-finite logits; the other rows are unaffected.
+ * The same call gives the same bits every time. A pipeline wait that runs out
+ * (nls_set_wait_limit) gives NLS_ERR_TIMEOUT and leaves y undefined.
+ * Workspace: the handle's, grown by the first call of a size (make that call
+ * before capturing the stream); it is never moved while the handle lives, so
+ * captured calls stay valid, but calls and replays on one handle must not
+ * overlap. Flags: NLS_DEVICE_INPUTS (x), NLS_DEVICE_OUTPUTS (y). */
+NLS_API nls_status nls_g4_matmul(nls_handle* h, const nls_g4_weights* w, const void* x,
+                                 int32_t xtype, int64_t ldx, int32_t nb, void* y, int32_t ytype,
+                                 int64_t ldy, uint32_t flags, void* stream);
+
+/* Settings of one row of nls_draw_batch: the members of nls_row_params that
+ * it uses, with the same meaning. 32 bytes, no padding. */
+typedef struct nls_draw_params {
+  double temperature; /* <= 0: the highest logit (the first of equal ones)      */
+  double top_p;       /* active iff 0 < top_p < 1                              */
+  double min_p;       /* active iff min_p > 0                                  */
+  int64_t top_k;      /* active iff 0 < top_k < vocab                          */
+} nls_draw_params;
+
+/* Draw one token per row from fp32, fp16 or bfloat16 logits. Per row, with the
+ * tokens in descending order of their logits (equal logits in ascending order
+ * of index) and masses m_i = exp((x_i - max x) / temperature):
+ *  1. top-k keeps the first top_k of that order;
+ *  2. top-p keeps the shortest prefix whose mass is at least top_p times the
+ *     mass of what top-k kept;
+ *  3. min-p keeps tokens with m_i >= min_p (the first token always);
+ *  4. the token is the first whose running mass is at least uniforms[r] times
+ *     the kept mass; its probability is m_i over the kept mass.
+ * This is nls_sample_batch's chain without penalties and bias, with the sums
+ * taken as real numbers (the masses in fixed point, 2^-45 of the largest,
+ * summed exactly) instead of the reference's sequential fp32 sums, and ties at
+ * the top-k border going to the lowest index.
+ *  logits    rows of vocab values of type ltype, ld >= vocab values apart,
+ *            aligned to their type
+ *  params    [rows]
+ *  uniforms  [rows] in [0, 1); NULL only if every row has temperature <= 0
+ *  out_ids   [rows]; out_probs [rows] or NULL (1 for temperature <= 0)
+ * A row that holds a NaN, whose maximum is +inf or that is -inf throughout
+ * gets id -1, probability 0 and NLS_ERR_NAN_LOGITS; a NaN temperature or a
+ * uniform outside [0, 1) gets id -1 and NLS_ERR_INVALID_ARG. -inf logits are
+ * never drawn. rows <= the handle's max_rows, vocab <= its max_vocab. Flags as
+ * nls_sample_batch. */
+NLS_API nls_status nls_draw_batch(nls_handle* h, const void* logits, int32_t ltype, int64_t ld,
+                                  int32_t rows, int32_t vocab, const nls_draw_params* params,
+                                  const double* uniforms, int64_t* out_ids, float* out_probs,
+                                  uint32_t flags, void* stream);
+
+/* The tail of a decode step: logits = nls_g4_matmul(w, x) of type ltype stay
+ * in the handle's device memory and nls_draw_batch draws from them. Arguments
+ * and flags as those two calls; rows <= the handle's max_rows and w->rows <=
+ * its max_vocab. */
+NLS_API nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, const void* x,
+                                       int32_t xtype, int64_t ldx, int32_t rows, int32_t ltype,
+                                       const nls_draw_params* params, const double* uniforms,
+                                       int64_t* out_ids, float* out_probs, uint32_t flags,
+                                       void* stream);
+
 /* Per-kernel timing of later calls on this handle (tracing; no counterpart
  * in the reference, which only times whole generations with epochTime,
  * chat.nim:191,246-247). With `on` set, every sampling call records CUDA

@@ -10,7 +10,8 @@ __graft_entry__.py (or register it yourself with importlib under the module
 name `nimllm_b200`).
 """
 from . import workloads
-from ._abi import EXPORTS, LIB_PATH, NlsError, ROW_PARAMS_DTYPE, load
+from ._abi import DRAW_PARAMS_DTYPE, EXPORTS, LIB_PATH, NlsError, ROW_PARAMS_DTYPE, load
+from .g4 import G4Weights, draw_params, g4_pack, g4_quantize
 from .sampler import (Comm, Engine, Rand, Sampler, SamplerParams, accept, argmax, batch_inputs,
                       comm_unique_id, decode_step_many, default_engine, defaultSampling,
                       greedySampling, newSampler, params_record, perplexity_from_logits,

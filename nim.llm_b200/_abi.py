@@ -35,12 +35,29 @@ EXPORTS = (
     "nls_top_tokens", "nls_token_nll", "nls_lm_head", "nls_lm_head_sample",
     "nls_device_upload", "nls_device_free", "nls_ref_expf_range", "nls_noalloc_status",
     "nls_set_wait_limit", "nls_comm_set_timeout", "nls_comm_abort",
+    "nls_g4_matmul", "nls_draw_batch", "nls_g4_lm_head_draw",
 )
 
 # ggml weight types of nls_lm_head (GgmlType codes, quant.nim:14-19)
 NLS_WT = {"f32": 0, "f16": 1, "q4_0": 2, "q8_0": 8, "q6_k": 14}
 NLS_EXACT_MATMUL = 4
 NLS_ROWS_INDEPENDENT = 8
+
+# element types of nls_g4_matmul and nls_draw_batch
+NLS_DT = {"f32": 0, "f16": 1, "bf16": 2}
+
+# nls_draw_params: 3 doubles + 1 int64, 32 bytes, no padding.
+DRAW_PARAMS_DTYPE = np.dtype([("temperature", "<f8"), ("top_p", "<f8"), ("min_p", "<f8"),
+                              ("top_k", "<i8")])
+assert DRAW_PARAMS_DTYPE.itemsize == 32
+
+
+class G4WeightsStruct(ctypes.Structure):
+    """nls_g4_weights."""
+    _fields_ = [("q", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("mins", ctypes.c_void_p),
+                ("q_ld", ctypes.c_int64), ("s_ld", ctypes.c_int64), ("rows", ctypes.c_int32),
+                ("cols", ctypes.c_int32), ("group", ctypes.c_int32), ("stype", ctypes.c_int32)]
+
 
 # nls_row_params: 6 doubles + 2 int64, 64 bytes, no padding.
 ROW_PARAMS_DTYPE = np.dtype([
@@ -117,6 +134,13 @@ def load(path: str | None = None):
     L.nls_noalloc_status.argtypes = [vp, u32, vp]
     L.nls_ref_expf_range.restype = i32
     L.nls_ref_expf_range.argtypes = [u32, i64, vp, vp, vp]
+    g4 = ctypes.POINTER(G4WeightsStruct)
+    L.nls_g4_matmul.restype = i32
+    L.nls_g4_matmul.argtypes = [vp, g4, vp, i32, i64, i32, vp, i32, i64, u32, vp]
+    L.nls_draw_batch.restype = i32
+    L.nls_draw_batch.argtypes = [vp, vp, i32, i64, i32, i32, vp, vp, vp, vp, u32, vp]
+    L.nls_g4_lm_head_draw.restype = i32
+    L.nls_g4_lm_head_draw.argtypes = [vp, g4, vp, i32, i64, i32, i32, vp, vp, vp, vp, u32, vp]
     _lib = L
     return L
 

@@ -13,7 +13,21 @@
 
 #include "nls_kernels.h"
 #include "nls_nccl.h"
+#include "nls_types.cuh"
 #include "nimllm_sample.h"
+
+namespace nls {
+// A device buffer that captured calls may keep using: growing it allocates a
+// new one and keeps the old one until the handle is destroyed.
+struct Workspace {
+  void* p = nullptr;
+  size_t cap = 0;
+};
+struct Retired {
+  void* p;
+  Retired* next;
+};
+}  // namespace nls
 
 struct nls_handle {
   int device = 0;
@@ -82,6 +96,11 @@ struct nls_handle {
   size_t lmq_cap = 0;
   float* d_lmy = nullptr;
   size_t lmy_cap = 0;
+  // nls_g4_matmul and nls_draw_batch: kernel workspace, host-staged inputs
+  // (activations or logits; params; uniforms), logits of the combined call and
+  // host-output results
+  nls::Workspace g4_ws, g4_x, g4_y, draw_x, draw_p, draw_u;
+  nls::Retired* retired = nullptr;
   char last_err[256] = {0};
 };
 
@@ -129,6 +148,42 @@ nls_status grow(nls_handle* h, T** p, size_t* cap, size_t n) {
   size_t want = n < 1024 ? 1024 : n;
   NLS_CUDA(h, cudaMalloc((void**)p, want * sizeof(T)));
   *cap = want;
+  return NLS_OK;
+}
+
+// At least `bytes` in w (see Workspace). A capturing stream must not allocate:
+// the call is refused and its capture left intact.
+nls_status ws_grow(nls_handle* h, nls::Workspace* w, size_t bytes, cudaStream_t st) {
+  if (bytes <= w->cap) return NLS_OK;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  NLS_CUDA(h, cudaStreamIsCapturing(st, &cap));
+  if (cap != cudaStreamCaptureStatusNone) {
+    snprintf(h->last_err, sizeof h->last_err,
+             "the stream is capturing and the workspace has to grow: make a call of this size first");
+    return NLS_ERR_CAPACITY;
+  }
+  nls::Retired* old = nullptr;
+  if (w->p) {
+    old = static_cast<nls::Retired*>(malloc(sizeof(nls::Retired)));
+    if (!old) return NLS_ERR_CAPACITY;
+  }
+  // (at least half again as much, so that growing step by step retires at
+  // most about twice the final size)
+  size_t want = bytes > w->cap + w->cap / 2 ? bytes : w->cap + w->cap / 2;
+  want = (want + 255) & ~size_t(255);
+  void* p = nullptr;
+  const cudaError_t e = cudaMalloc(&p, want);
+  if (e != cudaSuccess) {
+    free(old);
+    (void)cudaGetLastError();
+    return cuda_fail(h, e, "cudaMalloc (workspace)");
+  }
+  if (old) {
+    *old = nls::Retired{w->p, h->retired};
+    h->retired = old;
+  }
+  w->p = p;
+  w->cap = want;
   return NLS_OK;
 }
 
@@ -298,6 +353,12 @@ void nls_destroy(nls_handle* h) {
     cudaFree(h->d_lmx);
     cudaFree(h->d_lmq);
     cudaFree(h->d_lmy);
+    for (nls::Workspace* w : {&h->g4_ws, &h->g4_x, &h->g4_y, &h->draw_x, &h->draw_p, &h->draw_u}) cudaFree(w->p);
+    while (nls::Retired* r = h->retired) {
+      h->retired = r->next;
+      cudaFree(r->p);
+      free(r);
+    }
     if (h->fork) cudaEventDestroy(h->fork);
     if (h->join) cudaEventDestroy(h->join);
     for (cudaEvent_t e : h->ev)
@@ -592,6 +653,174 @@ nls_status nls_lm_head_sample(nls_handle* h, const void* weights, int32_t wtype,
   return sample_impl(h, h->d_logits, vocab, true, true, rows, vocab, params, hist_ids, hist_off,
                      bias_ids, bias_vals, bias_off, uniforms, out_ids, out_probs,
                      flags & ~(NLS_EXACT_MATMUL | NLS_ROWS_INDEPENDENT), st);
+}
+
+}  // extern "C"
+
+namespace {
+
+bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+bool g4_weights_ok(const nls_g4_weights* w) {
+  if (!w || !w->q || !w->scales) return false;
+  if (!aligned_to(w->q, 16) || !aligned_to(w->scales, 16) || !aligned_to(w->mins, 16)) return false;
+  if (w->rows < 1 || w->cols < 32 || w->cols % 32 != 0 || !nls::dt_ok(w->stype)) return false;
+  if (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128 != 0)) return false;
+  return w->q_ld % 16 == 0 && w->q_ld >= w->cols / 2 && w->s_ld % 8 == 0 && w->s_ld >= w->rows;
+}
+
+// The product into device memory dy; clears and then uses d_work[0].
+nls_status g4_impl(nls_handle* h, const nls_g4_weights* w, const void* x, int32_t xtype, int64_t ldx,
+                   bool x_dev, int32_t nb, void* dy, int32_t ytype, int64_t ldy, cudaStream_t st) {
+  nls_status s;
+  nls::G4Args a{};
+  a.q = w->q;
+  a.scales = w->scales;
+  a.mins = w->mins;
+  a.q_ld = w->q_ld;
+  a.s_ld = w->s_ld;
+  a.rows = w->rows;
+  a.cols = w->cols;
+  a.group = w->group;
+  a.stype = w->stype;
+  a.x = x;
+  a.xtype = xtype;
+  a.ldx = ldx;
+  a.nb = nb;
+  a.y = dy;
+  a.ytype = ytype;
+  a.ldy = ldy;
+  a.status = h->d_work;
+  a.wait_ns = h->wait_ns;
+  if (!x_dev) {
+    const size_t es = nls::dt_size(xtype), line = (size_t)w->cols * es;
+    if ((s = ws_grow(h, &h->g4_x, (size_t)nb * line, st)) != NLS_OK) return s;
+    NLS_CUDA(h, cudaMemcpy2DAsync(h->g4_x.p, line, x, (size_t)ldx * es, line, nb, cudaMemcpyHostToDevice, st));
+    a.x = h->g4_x.p;
+    a.ldx = w->cols;
+  }
+  if ((s = ws_grow(h, &h->g4_ws, nls::g4_workspace_bytes(a, h->sm_count), st)) != NLS_OK) return s;
+  NLS_CUDA(h, nls::launch_g4(a, h->g4_ws.p, h->sm_count, st));
+  return NLS_OK;
+}
+
+// nls_draw_batch after its argument checks; d_work[0] is the caller's.
+nls_status draw_impl(nls_handle* h, const void* logits, int32_t ltype, int64_t ld, bool logits_dev,
+                     int32_t rows, int32_t vocab, const nls_draw_params* params,
+                     const double* uniforms, int64_t* out_ids, float* out_probs, uint32_t flags,
+                     cudaStream_t st) {
+  const bool dev_in = (flags & NLS_DEVICE_INPUTS) != 0, dev_out = (flags & NLS_DEVICE_OUTPUTS) != 0;
+  nls_status s;
+  nls::DrawArgs a{};
+  a.logits = logits;
+  a.ltype = ltype;
+  a.ld = ld;
+  a.rows = rows;
+  a.V = vocab;
+  a.params = params;
+  a.uniforms = uniforms;
+  a.status = h->d_work;
+  if (!logits_dev) {
+    const size_t es = nls::dt_size(ltype), line = (size_t)vocab * es;
+    if ((s = ws_grow(h, &h->draw_x, (size_t)rows * line, st)) != NLS_OK) return s;
+    NLS_CUDA(h, cudaMemcpy2DAsync(h->draw_x.p, line, logits, (size_t)ld * es, line, rows,
+                                  cudaMemcpyHostToDevice, st));
+    a.logits = h->draw_x.p;
+    a.ld = vocab;
+  }
+  if (!dev_in) {
+    if ((s = ws_grow(h, &h->draw_p, sizeof(nls_draw_params) * (size_t)h->max_rows, st)) != NLS_OK) return s;
+    NLS_CUDA(h, cudaMemcpyAsync(h->draw_p.p, params, sizeof(nls_draw_params) * (size_t)rows,
+                                cudaMemcpyHostToDevice, st));
+    a.params = static_cast<const nls_draw_params*>(h->draw_p.p);
+    if (uniforms) {
+      if ((s = ws_grow(h, &h->draw_u, sizeof(double) * (size_t)h->max_rows, st)) != NLS_OK) return s;
+      NLS_CUDA(h, cudaMemcpyAsync(h->draw_u.p, uniforms, sizeof(double) * (size_t)rows,
+                                  cudaMemcpyHostToDevice, st));
+      a.uniforms = static_cast<const double*>(h->draw_u.p);
+    }
+  }
+  a.out_ids = dev_out ? out_ids : h->d_out_ids;
+  a.out_probs = dev_out ? out_probs : (out_probs ? h->d_out_probs : nullptr);
+  NLS_CUDA(h, nls::launch_draw(a, h->sm_count, st));
+  if (dev_out) return NLS_OK;
+  NLS_CUDA(h, cudaMemcpyAsync(h->h_status, h->d_work, sizeof(int), cudaMemcpyDeviceToHost, st));
+  NLS_CUDA(h, cudaMemcpyAsync(out_ids, h->d_out_ids, sizeof(int64_t) * rows, cudaMemcpyDeviceToHost, st));
+  if (out_probs)
+    NLS_CUDA(h, cudaMemcpyAsync(out_probs, h->d_out_probs, sizeof(float) * rows, cudaMemcpyDeviceToHost, st));
+  NLS_CUDA(h, cudaStreamSynchronize(st));
+  return (nls_status)*h->h_status;
+}
+
+constexpr uint32_t kDevFlags = NLS_DEVICE_INPUTS | NLS_DEVICE_OUTPUTS;
+
+}  // namespace
+
+extern "C" {
+
+nls_status nls_g4_matmul(nls_handle* h, const nls_g4_weights* w, const void* x, int32_t xtype,
+                         int64_t ldx, int32_t nb, void* y, int32_t ytype, int64_t ldy,
+                         uint32_t flags, void* stream) {
+  if (!h || (flags & ~kDevFlags) || nb < 0) return NLS_ERR_INVALID_ARG;
+  if (!g4_weights_ok(w) || !nls::dt_ok(xtype) || !nls::dt_ok(ytype)) return NLS_ERR_INVALID_ARG;
+  if (ldx < w->cols || ldy < w->rows) return NLS_ERR_INVALID_ARG;
+  if (nb == 0) return NLS_OK;
+  if (!x || !y || !aligned_to(x, nls::dt_size(xtype)) || !aligned_to(y, nls::dt_size(ytype)))
+    return NLS_ERR_INVALID_ARG;
+  DeviceGuard g(h->device);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool dev_out = (flags & NLS_DEVICE_OUTPUTS) != 0;
+  nls_status s;
+  void* dy = y;
+  int64_t dld = ldy;
+  const size_t es = nls::dt_size(ytype), line = (size_t)w->rows * es;
+  if (!dev_out) {
+    if ((s = ws_grow(h, &h->g4_y, (size_t)nb * line, st)) != NLS_OK) return s;
+    dy = h->g4_y.p;
+    dld = w->rows;
+  }
+  if ((s = g4_impl(h, w, x, xtype, ldx, (flags & NLS_DEVICE_INPUTS) != 0, nb, dy, ytype, dld, st)) != NLS_OK)
+    return s;
+  if (dev_out) return NLS_OK;
+  NLS_CUDA(h, cudaMemcpyAsync(h->h_status, h->d_work, sizeof(int), cudaMemcpyDeviceToHost, st));
+  NLS_CUDA(h, cudaMemcpy2DAsync(y, (size_t)ldy * es, dy, line, line, nb, cudaMemcpyDeviceToHost, st));
+  NLS_CUDA(h, cudaStreamSynchronize(st));
+  return (nls_status)*h->h_status;
+}
+
+nls_status nls_draw_batch(nls_handle* h, const void* logits, int32_t ltype, int64_t ld, int32_t rows,
+                          int32_t vocab, const nls_draw_params* params, const double* uniforms,
+                          int64_t* out_ids, float* out_probs, uint32_t flags, void* stream) {
+  if (!h || (flags & ~kDevFlags)) return NLS_ERR_INVALID_ARG;
+  if (rows < 0 || vocab < 1 || ld < vocab || !nls::dt_ok(ltype)) return NLS_ERR_INVALID_ARG;
+  if (rows == 0) return NLS_OK;
+  if (!logits || !aligned_to(logits, nls::dt_size(ltype)) || !params || !out_ids) return NLS_ERR_INVALID_ARG;
+  if (rows > h->max_rows || vocab > h->max_vocab) return NLS_ERR_CAPACITY;
+  DeviceGuard g(h->device);
+  cudaStream_t st = (cudaStream_t)stream;
+  NLS_CUDA(h, cudaMemsetAsync(h->d_work, 0, sizeof(int), st));
+  return draw_impl(h, logits, ltype, ld, (flags & NLS_DEVICE_INPUTS) != 0, rows, vocab, params, uniforms,
+                   out_ids, out_probs, flags, st);
+}
+
+nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, const void* x, int32_t xtype,
+                               int64_t ldx, int32_t rows, int32_t ltype, const nls_draw_params* params,
+                               const double* uniforms, int64_t* out_ids, float* out_probs,
+                               uint32_t flags, void* stream) {
+  if (!h || (flags & ~kDevFlags) || rows < 0) return NLS_ERR_INVALID_ARG;
+  if (!g4_weights_ok(w) || !nls::dt_ok(xtype) || !nls::dt_ok(ltype) || ldx < w->cols) return NLS_ERR_INVALID_ARG;
+  if (rows == 0) return NLS_OK;
+  if (!x || !aligned_to(x, nls::dt_size(xtype)) || !params || !out_ids) return NLS_ERR_INVALID_ARG;
+  if (rows > h->max_rows || w->rows > h->max_vocab) return NLS_ERR_CAPACITY;
+  DeviceGuard g(h->device);
+  cudaStream_t st = (cudaStream_t)stream;
+  nls_status s;
+  // logits rows 16-byte aligned
+  const int64_t ld = ((int64_t)w->rows + 7) & ~int64_t(7);
+  if ((s = ws_grow(h, &h->g4_y, (size_t)rows * ld * nls::dt_size(ltype), st)) != NLS_OK) return s;
+  if ((s = g4_impl(h, w, x, xtype, ldx, (flags & NLS_DEVICE_INPUTS) != 0, rows, h->g4_y.p, ltype, ld, st)) != NLS_OK)
+    return s;
+  return draw_impl(h, h->g4_y.p, ltype, ld, true, rows, w->rows, params, uniforms, out_ids, out_probs, flags, st);
 }
 
 nls_status nls_argmax_batch(nls_handle* h, const float* logits, int64_t ld, int32_t rows,

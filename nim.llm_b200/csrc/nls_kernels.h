@@ -69,4 +69,39 @@ size_t lm_head_act_scratch_bytes(int cols);
 cudaError_t launch_lm_head_mma(const uint8_t* w, int wtype, int64_t row_bytes, int rows, int cols, const float* x,
                                int nb, float* y, int64_t ldy, int* status, int sm_count,
                                unsigned long long wait_ns, uint8_t* act_scratch, cudaStream_t st);
+
+// 4-bit weights with group scales (nls_g4_matmul); all pointers device memory.
+struct G4Args {
+  const void* q;
+  const void* scales;
+  const void* mins;  // may be null
+  int64_t q_ld, s_ld;
+  int rows, cols, group, stype;
+  const void* x;
+  int xtype;
+  int64_t ldx;
+  int nb;
+  void* y;
+  int ytype;
+  int64_t ldy;
+  int* status;  // cleared by the launch, then as the other kernels' status
+  unsigned long long wait_ns;
+};
+// bytes of device workspace launch_g4 needs for these arguments
+size_t g4_workspace_bytes(const G4Args& a, int sm_count);
+cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream_t st);
+
+// Drawing tokens from logits of any type (nls_draw_batch).
+struct DrawArgs {
+  const void* logits;
+  int ltype;
+  int64_t ld;
+  int rows, V;
+  const nls_draw_params* params;
+  const double* uniforms;  // may be null
+  int64_t* out_ids;
+  float* out_probs;  // may be null
+  int* status;
+};
+cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st);
 }  // namespace nls

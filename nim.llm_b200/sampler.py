@@ -14,6 +14,7 @@ torch CUDA tensors (device memory, NLS_DEVICE_INPUTS).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 from typing import Optional
@@ -21,7 +22,8 @@ from typing import Optional
 import numpy as np
 
 from . import _abi
-from ._abi import NlsError, ROW_PARAMS_DTYPE
+from . import g4 as _g4
+from ._abi import DRAW_PARAMS_DTYPE, NlsError, ROW_PARAMS_DTYPE
 
 
 # ---------------------------------------------------------------------------
@@ -331,6 +333,162 @@ class Engine:
         if check:
             self._check(st, "nls_lm_head_sample")
         return ids, probs, st
+
+    # -- 4-bit weights with group scales, and drawing from typed logits -------
+    def _on(self, cuda: bool, stream):
+        """Context of a call: for CUDA tensors the engine's device and the
+        given stream (None: torch's current one), on which temporaries are made
+        and results allocated."""
+        if not cuda:
+            return contextlib.nullcontext()
+        import torch
+        dev = torch.device("cuda", self.device)
+        return torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else
+                                 torch.cuda.ExternalStream(int(stream), device=dev))
+
+    def _stream(self, cuda: bool, stream):
+        if not cuda:
+            return ctypes.c_void_p(0 if stream is None else int(stream))
+        import torch
+        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _finish(self, st: int, what: str, cuda: bool, stream, check: bool) -> int:
+        """Raise on a call's error. Arguments and launches are always checked;
+        the kernels' status of a device call only with `check` (it waits)."""
+        if st != 0 and (check or cuda):
+            self._check(st, what)
+        if cuda and check:
+            st = self._lib.nls_stream_status(self._h, stream)
+            self._check(st, f"{what} (kernel status)")
+        return st
+
+    def _g4_weights(self, w):
+        if w.device.type != "cuda" or w.device.index != self.device:
+            raise ValueError(f"the weights are on {w.device}, the engine on cuda:{self.device}")
+        return ctypes.byref(w.struct)
+
+    @staticmethod
+    def _g4_x(w, x):
+        """x as [nb, cols] with contiguous rows."""
+        x = x[None, :] if x.dim() == 1 else x
+        if x.dim() != 2 or x.shape[1] != w.cols:
+            raise ValueError(f"x must be [nb, {w.cols}]")
+        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < w.cols):
+            x = x.contiguous()
+        return x
+
+    def g4_matmul(self, w, x, out=None, out_dtype=None, stream=None, check: bool = True):
+        """x . W^T for 4-bit weights (G4Weights): [nb, rows] of `out_dtype` (x's
+        by default). x [nb, cols] or [cols], a CUDA tensor (stream-ordered on
+        `stream`, torch's current one by default; check=False does not wait for
+        the kernels) or a CPU tensor (returns a CPU tensor)."""
+        import torch
+        cuda = x.is_cuda
+        weights = self._g4_weights(w)
+        with self._on(cuda, stream):
+            x2 = self._g4_x(w, x)
+            nb = x2.shape[0]
+            if out is not None and out_dtype is not None and out.dtype != out_dtype:
+                raise ValueError("out is not of out_dtype")
+            if out is None:
+                y = torch.empty((nb, w.rows), dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+            else:
+                y = out[None, :] if out.dim() == 1 else out
+            if tuple(y.shape) != (nb, w.rows):
+                raise ValueError(f"out must be [{nb}, {w.rows}]")
+            dev = self.device if cuda else None
+            xp, ldx = _g4.rows_of(x2, dev, "x")
+            yp, ldy = _g4.rows_of(y, dev, "out")
+            sp = self._stream(cuda, stream)
+            st = self._lib.nls_g4_matmul(
+                self._h, weights, xp, _g4.dt_code(x.dtype), ldx, nb, yp, _g4.dt_code(y.dtype), ldy,
+                _abi.NLS_DEVICE_INPUTS | _abi.NLS_DEVICE_OUTPUTS if cuda else 0, sp)
+            self._finish(st, "nls_g4_matmul", cuda, sp, check)
+        return out if out is not None else (y[0] if x.dim() == 1 else y)
+
+    def _draw_inputs(self, B, params, uniforms, out_ids, out_probs, cuda):
+        """(params, uniforms, ids, probs, then their pointers) of a draw."""
+        import torch
+        if not cuda:
+            params = np.ascontiguousarray(params, dtype=DRAW_PARAMS_DTYPE)
+            if params.shape != (B,):
+                raise ValueError("one params record per row")
+            if uniforms is not None:
+                uniforms = np.ascontiguousarray(uniforms, dtype=np.float64)
+                if uniforms.shape != (B,):
+                    raise ValueError("one uniform per row")
+            ids = np.empty(B, np.int64) if out_ids is None else out_ids
+            probs = np.empty(B, np.float32) if out_probs is None else out_probs
+            for a, dt, what in ((ids, np.int64, "out_ids"), (probs, np.float32, "out_probs")):
+                if not isinstance(a, np.ndarray) or a.dtype != dt or a.shape != (B,) or not a.flags.c_contiguous:
+                    raise ValueError(f"{what}: {B} contiguous {np.dtype(dt).name} expected")
+            return (params, uniforms, ids, probs, _host_ptr(params), _host_ptr(uniforms), _host_ptr(ids),
+                    _host_ptr(probs))
+        dev = torch.device("cuda", self.device)
+        if not _is_torch(params):
+            params = torch.from_numpy(np.ascontiguousarray(params, dtype=DRAW_PARAMS_DTYPE).view(np.uint8)).to(dev)
+        if uniforms is not None and not _is_torch(uniforms):
+            uniforms = torch.from_numpy(np.ascontiguousarray(uniforms, dtype=np.float64)).to(dev)
+        if params.device != dev or not params.is_contiguous() or params.numel() * params.element_size() != 32 * B:
+            raise ValueError(f"params: a contiguous tensor of 32 bytes per row on {dev} expected")
+        ids = torch.empty(B, dtype=torch.int64, device=dev) if out_ids is None else out_ids
+        probs = torch.empty(B, dtype=torch.float32, device=dev) if out_probs is None else out_probs
+        for t, dt, what in ((uniforms, torch.float64, "uniforms"), (ids, torch.int64, "out_ids"),
+                            (probs, torch.float32, "out_probs")):
+            if t is not None and (t.device != dev or t.dtype != dt or not t.is_contiguous() or t.numel() != B):
+                raise ValueError(f"{what}: {B} contiguous {dt} on {dev} expected")
+        ptr = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        return params, uniforms, ids, probs, ptr(params), ptr(uniforms), ptr(ids), ptr(probs)
+
+    def draw_batch(self, logits, params, uniforms=None, out_ids=None, out_probs=None, stream=None,
+                   check: bool = True):
+        """Draw one token per row of float32, float16 or bfloat16 logits [B, V]
+        (nls_draw_batch): returns (ids int64 [B], probs float32 [B], status).
+
+        CUDA tensor: params (draw_params records, or a device tensor of 32
+        bytes per row) and float64 uniforms; results are CUDA tensors, the call
+        is stream-ordered (check=False does not wait). CPU tensor or numpy
+        array: numpy params, uniforms and results."""
+        import torch
+        if not _is_torch(logits):
+            logits = torch.from_numpy(np.ascontiguousarray(logits))
+        cuda = logits.is_cuda
+        with self._on(cuda, stream):
+            if logits.dim() == 1:
+                logits = logits[None, :]
+            if logits.dim() != 2:
+                raise ValueError("logits must be [B, V]")
+            B, V = logits.shape
+            if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
+                logits = logits.contiguous()
+            xp, ld = _g4.rows_of(logits, self.device if cuda else None, "logits")
+            hold = self._draw_inputs(B, params, uniforms, out_ids, out_probs, cuda)
+            sp = self._stream(cuda, stream)
+            st = self._lib.nls_draw_batch(
+                self._h, xp, _g4.dt_code(logits.dtype), ld, B, V, *hold[4:],
+                _abi.NLS_DEVICE_INPUTS | _abi.NLS_DEVICE_OUTPUTS if cuda else 0, sp)
+            st = self._finish(st, "nls_draw_batch", cuda, sp, check)
+        return hold[2], hold[3], st
+
+    def g4_lm_head_draw(self, w, x, params, uniforms=None, logits_dtype=None, out_ids=None, out_probs=None,
+                        stream=None, check: bool = True):
+        """The tail of a decode step: g4_matmul(w, x) into logits of
+        `logits_dtype` (x's by default) that stay in the handle's memory, then
+        draw_batch from them. x [B, cols], CUDA or CPU; results as draw_batch."""
+        cuda = x.is_cuda
+        weights = self._g4_weights(w)
+        with self._on(cuda, stream):
+            x = self._g4_x(w, x)
+            B = x.shape[0]
+            xp, ldx = _g4.rows_of(x, self.device if cuda else None, "x")
+            hold = self._draw_inputs(B, params, uniforms, out_ids, out_probs, cuda)
+            sp = self._stream(cuda, stream)
+            st = self._lib.nls_g4_lm_head_draw(
+                self._h, weights, xp, _g4.dt_code(x.dtype), ldx, B,
+                _g4.dt_code(x.dtype if logits_dtype is None else logits_dtype), *hold[4:],
+                _abi.NLS_DEVICE_INPUTS | _abi.NLS_DEVICE_OUTPUTS if cuda else 0, sp)
+            st = self._finish(st, "nls_g4_lm_head_draw", cuda, sp, check)
+        return hold[2], hold[3], st
 
     def argmax_batch(self, logits) -> np.ndarray:
         logits = np.ascontiguousarray(np.asarray(logits, dtype=np.float32))
