@@ -336,3 +336,45 @@ def test_device_refusals(pkg, eng):
         eng.g4_matmul(w, x, out=torch.empty((2, 64)))
     with pytest.raises(TypeError):
         eng.g4_matmul(w, x.double())
+
+
+@pytest.mark.gpu
+def test_capture_that_would_have_to_allocate(pkg, eng):
+    """Refused, and the capture goes on."""
+    import torch
+    w = make(pkg, 3001, 1024, 128, "f16", False, seed=1)
+    x = torch.randn((2, 1024), device="cuda").half()
+    out = torch.empty((2, 3001), dtype=torch.float16, device="cuda")
+    other = pkg.Engine(0, max_rows=8, max_vocab=4096)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            with pytest.raises(pkg.NlsError) as e:
+                other.g4_matmul(w, x, out=out, check=False)
+            out.zero_()
+        assert e.value.status == pkg._abi.NLS_ERR_CAPACITY
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not bool(out.any())
+        check(w, x, other.g4_matmul(w, x))
+    finally:
+        del graph
+        other.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,nb", [(3001, 4096, 2), (40000, 512, 20)])
+def test_a_wait_that_runs_out_is_an_error(pkg, eng, rows, cols, nb):
+    import torch
+    w = make(pkg, rows, cols, 128, "f16", True, seed=3)
+    x = torch.randn((nb, cols), generator=torch.Generator().manual_seed(3)).half().cuda()
+    want = eng.g4_matmul(w, x)
+    for _ in range(2):
+        eng.set_wait_limit(0)
+        try:
+            with pytest.raises(pkg.NlsError) as e:
+                eng.g4_matmul(w, x)
+        finally:
+            eng.set_wait_limit(200 * 1000 * 1000)
+        assert e.value.status == pkg._abi.NLS_ERR_TIMEOUT
+        assert torch.equal(eng.g4_matmul(w, x), want)
