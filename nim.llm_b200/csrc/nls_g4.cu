@@ -30,12 +30,13 @@
 // shape; a tile that more than one CTA worked on is joined by the last of them
 // to finish, from partial sums in the workspace added in CTA order (the same
 // bits every time; no CTA waits for another).
-// One CTA: 16 worker warps (warp w: lanes 32 (w & 3) .. of tile half (w >> 2)
-// & 1, columns of half w >> 3 of the step and of the batch) and one warp that
-// issues the copies (a ring of stages: packed weights by tensor map,
-// activations, scales) and the MMAs. Workers unpack step s while the MMAs of
-// step s - 1 run, then add step s - 1's sums; operands and accumulators are
-// double-buffered in TMEM (2 x 128 and 2 x 128 columns).
+// One CTA: 16 worker warps in two sets, one that issues the copies (a ring of
+// stages: packed weights by tensor map, activations, scales) and one that
+// issues the MMAs. A set unpacks every other step (a thread 128 columns of its
+// row, so the waits, scales and bookkeeping of a step come once per 128
+// weights) and adds its half of the batch columns of every step's sums; while
+// one set unpacks, the other's MMAs run. Operands and accumulators have one
+// buffer per set in TMEM (2 x 128 and 2 x 128 columns).
 #include <cuda.h>
 
 #include <algorithm>
@@ -52,22 +53,25 @@ namespace {
 
 constexpr int kTile = 256;       // weight rows per tile
 constexpr int kStep = 128;       // columns per step
-constexpr int kWorkers = 16;     // warps
-constexpr int kThreads = 32 * (kWorkers + 1);
+constexpr int kWorkers = 16;     // warps, in two sets
+constexpr int kCopyWarp = kWorkers, kMmaWarp = kWorkers + 1;
+constexpr int kThreads = 32 * (kWorkers + 2);
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemD = 256;  // A buffers below, accumulators from here on
 
-// MMA columns of a launch of nb batch rows, and batch rows per worker thread
-// (a worker takes one half of them)
+// batch rows per worker thread of a launch of nb (a set takes one half of
+// them), and the MMA's columns
 __host__ __device__ constexpr int cols_per_thread(int nb) {
   return nb <= 2 ? 1 : nb <= 4 ? 2 : nb <= 8 ? 4 : nb <= 16 ? 8 : nb <= 32 ? 16 : nb <= 48 ? 24 : 32;
 }
 __host__ __device__ constexpr int mma_n(int cpt) { return cpt <= 8 ? 16 : 2 * cpt; }
 // groups (scales) per step, and the most batch rows a launch takes with them:
 // each has 64 / regions accumulator columns of the 64 a tile half's buffer holds
+// fp32 activations' parts as columns of their own: up to 4 batch rows
+__host__ __device__ constexpr bool folded(int parts, int nb) { return parts == 3 && nb <= 4; }
 __host__ __device__ constexpr int regions_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
 
 struct Plan {
@@ -127,7 +131,7 @@ struct KernelArgs {
 // first block clears the status and the tiles' counters.
 template <class X>
 __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx, int nb, int n_cols, int cols,
-                                                         int parts, int regions, uint8_t* op, float* xsum,
+                                                         int parts, int fold, int regions, uint8_t* op, float* xsum,
                                                          int* count, int tiles, int* status, int clear_status) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int k = blockIdx.x, n = threadIdx.x >> 4, word = threadIdx.x & 15;
@@ -161,8 +165,15 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
     if (word % lanes == 0) xsum[((size_t)k * regions + word / lanes) * n_cols + n] = s;
   }
   constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-  uint8_t* dst = op + (size_t)k * parts * n_cols * (kStep * 2) + (size_t)(word >> 1) * (n_cols * 32) +
-                 (n >> 3) * 256 + (word & 1) * 128 + (n & 7) * 16;
+  // fold > 0: part p of batch row n is column p * fold + n (columns past the
+  // parts are zeros: threads n >= fold write them)
+  uint8_t* dst = op + (size_t)k * (fold ? 1 : parts) * n_cols * (kStep * 2) + (size_t)(word >> 1) * (n_cols * 32) +
+                 (word & 1) * 128;
+  auto line = [&](int c) { return dst + (c >> 3) * 256 + (c & 7) * 16; };
+  if (fold && n >= fold) {
+    if (n >= 3 * fold) *reinterpret_cast<uint4*>(line(n)) = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
 #pragma unroll
   for (int part = 0; part < (kF32 ? 3 : 1); ++part) {
     uint32_t w[4];
@@ -187,7 +198,8 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
       }
       w[j] = h[0] | (h[1] << 16);
     }
-    *reinterpret_cast<uint4*>(dst + (size_t)part * n_cols * (kStep * 2)) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint8_t* at = fold ? line(part * fold + n) : line(n) + (size_t)part * n_cols * (kStep * 2);
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -201,14 +213,28 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// D (+)= A . B^T, A in tensor memory, B by descriptor
-__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D (+)= A . B^T by the warp's leader, A in tensor memory, B by descriptor. The
+// whole warp gets here with the same values: behind a branch of one lane the
+// operands would have to be moved to uniform registers one by one, which made
+// an issue cost about 110 cycles.
+template <bool ACC>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %4, 0;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(leader), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t (&r)[32]) {
@@ -246,29 +272,41 @@ __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t* r) {
 // plus q, exactly; fp16's 10 bits of mantissa take the nibble at bit 4 too, as
 // 2^10 + 16 q
 template <bool BF16>
-__device__ __forceinline__ void unpack8(uint32_t w, uint32_t* o) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 c = __floats2bfloat162_rn(136.0f, 136.0f);
+struct Unpack {
+  // the power of two's bits, out of the compiler's sight: as an immediate it
+  // would take a logical operation of its own beside the mask's
+  uint32_t magic;
+  __device__ __forceinline__ Unpack() { asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400)); }
+  template <uint32_t MASK>
+  __device__ __forceinline__ uint32_t put(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));  // (w & MASK) | magic
+    return r;
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* o) const {
+    if constexpr (BF16) {
+      const __nv_bfloat162 c = __floats2bfloat162_rn(136.0f, 136.0f);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t t = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), c);
-      o[j] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  } else {
-    const __half2 c = __floats2half2_rn(1032.0f, 1032.0f);
-    const __half2 k = __floats2half2_rn(0.0625f, 0.0625f), d = __floats2half2_rn(-72.0f, -72.0f);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t t = put<0x000F000Fu>(w >> (4 * j));
+        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), c);
+        o[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    } else {
+      const __half2 c = __floats2half2_rn(1032.0f, 1032.0f);
+      const __half2 k = __floats2half2_rn(0.0625f, 0.0625f), d = __floats2half2_rn(-72.0f, -72.0f);
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const uint32_t v = w >> (4 * j);
-      const uint32_t t0 = (v & 0x000F000Fu) | 0x64006400u, t1 = (v & 0x00F000F0u) | 0x64006400u;
-      const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&t0), c);
-      const __half2 h1 = __hfma2(*reinterpret_cast<const __half2*>(&t1), k, d);
-      o[j] = *reinterpret_cast<const uint32_t*>(&h0);
-      o[j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+      for (int j = 0; j < 4; j += 2) {
+        const uint32_t v = w >> (4 * j);
+        const uint32_t t0 = put<0x000F000Fu>(v), t1 = put<0x00F000F0u>(v);
+        const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&t0), c);
+        const __half2 h1 = __hfma2(*reinterpret_cast<const __half2*>(&t1), k, d);
+        o[j] = *reinterpret_cast<const uint32_t*>(&h0);
+        o[j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+      }
     }
   }
-}
+};
 
 __device__ __forceinline__ float ld_scale(const uint8_t* base, int stype, int i) {
   if (stype == NLS_DT_F32) return reinterpret_cast<const float*>(base)[i];
@@ -284,18 +322,31 @@ __device__ __forceinline__ void st_out(void* y, int ytype, int64_t i, float v) {
 
 struct Bars {
   uint64_t full[kMaxStages];  // stage landed
-  uint64_t ready[2];          // every worker has stored step s's operand (s & 1)
-  uint64_t done[2];           // step s's MMAs have completed
+  uint64_t free[kMaxStages];  // every worker has added the step's sums (its MMAs are done, its scales read)
+  uint64_t ready[2];          // the set has stored its step's operand
+  uint64_t done[2];           // the step's MMAs have completed
   uint64_t joined;            // every worker has written its partial sums
   uint64_t told;              // whether this CTA is the tile's last
   uint32_t tmem;
   int fail, staged, issued, last;
 };
 
-template <bool BF16, int CPT, int R>
+// a whole warp's bounded wait (the same answer in every lane)
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
+  if (limit_ns == 0) return false;
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return !__any_sync(0xffffffffu, !mbar_wait_bounded(bar, parity, limit_ns));
+}
+
+// CPT: batch rows per thread. R: groups per step. FOLD: the three parts of fp32
+// activations are columns of their own (part p of batch row b in column
+// 2 CPT p + b), else further MMAs into the same columns.
+template <bool BF16, int CPT, int R, bool FOLD>
 __global__ void __launch_bounds__(kThreads, 1)
     g4_kernel(const KernelArgs a, const __grid_constant__ CUtensorMap qmap) {
   constexpr int N = mma_n(CPT);
+  constexpr int P = FOLD ? 3 : 1;
+  static_assert(2 * CPT * P <= N && R * N <= 64, "columns");
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars& B = *reinterpret_cast<Bars*>(smem + (size_t)a.stages * a.stage_bytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -304,9 +355,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tile0 = (int)(s0 / a.ksteps), k0 = (int)(s0 % a.ksteps);
 
   if (tid == 0) {
-    for (int i = 0; i < kMaxStages; ++i) mbar_init(&B.full[i], 1);
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(&B.full[i], 1);
+      mbar_init(&B.free[i], kWorkers);
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B.ready[i], kWorkers);
+      mbar_init(&B.ready[i], kWorkers / 2);
       mbar_init(&B.done[i], 1);
     }
     mbar_init(&B.joined, kWorkers);
@@ -315,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     B.staged = B.issued = -1;
     fence_mbar_init();
   }
-  if (warp == kWorkers) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)),
                  "r"(kTmemCols)
                  : "memory");
@@ -329,15 +383,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   bool fail = false;
-  if (warp == kWorkers) {
+  if (warp == kCopyWarp) {
     if (lane == 0) {
-      int ltile = tile0, lk = k0;  // position of the next step to stage
-      auto stage = [&](int s) {
-        if (s >= nsteps) return;
-        uint8_t* st = smem + (size_t)(s % a.stages) * a.stage_bytes;
-        uint64_t* bar = &B.full[s % a.stages];
-        const int r0 = ltile * kTile, g0 = (int)((int64_t)lk * kStep / a.group);
-        const uint32_t xb = (uint32_t)(a.parts * N * kStep * 2);
+      // position of the next step; its stage and the phase its last step left
+      // there; its group and, where groups are wider than a step, the steps
+      // left in it
+      int ltile = tile0, lk = k0, slot = 0;
+      uint32_t phase = 1;
+      const int per = R == 1 ? a.group / kStep : 1;
+      int g0 = R == 1 ? k0 / per : k0 * R, left = per - (R == 1 ? k0 % per : 0);
+      const uint32_t xb = (uint32_t)(a.parts * N * kStep * 2);
+      for (int s = 0; s < nsteps; ++s) {
+        if (s >= a.stages && !mbar_wait_bounded(&B.free[slot], phase, a.wait_ns)) {
+          fail = true;
+          break;
+        }
+        uint8_t* st = smem + (size_t)slot * a.stage_bytes;
+        uint64_t* bar = &B.full[slot];
+        const int r0 = ltile * kTile;
         const uint32_t line = (uint32_t)(min(kTile, (a.rows - r0 + 7) & ~7) * a.ssize);
         const int ng = min(R, a.ngroups - g0);
         mbar_arrive_expect_tx(bar, kRawBytes + xb + (uint32_t)ng * line * (a.mins ? 2u : 1u));
@@ -350,87 +413,140 @@ __global__ void __launch_bounds__(kThreads, 1)
             bulk_copy_g2s(st + a.m_off + g * kTile * a.ssize, static_cast<const uint8_t*>(a.mins) + at, line, bar);
         }
         B.staged = s;
+        if (++slot == a.stages) {
+          slot = 0;
+          phase ^= 1;
+        }
+        if (R > 1) {
+          g0 += R;
+        } else if (--left == 0) {
+          left = per;
+          ++g0;
+        }
         if (++lk == a.ksteps) {
           lk = 0;
           ++ltile;
-        }
-      };
-      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
-                             ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-      for (int s = 0; s < a.stages; ++s) stage(s);
-      for (int s = 0; s < nsteps; ++s) {
-        if (!mbar_wait_bounded(&B.ready[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns)) {
-          fail = true;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t xs = smem_u32(smem) + (uint32_t)((s % a.stages) * a.stage_bytes + a.x_off);
-        // no-swizzle K-major descriptor: 128 bytes from a row's first 8
-        // columns to its next 8, 256 from 8 rows to the next
-        const uint64_t bd = (uint64_t)((xs >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) |
-                            ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46);
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t ta = tbase + (uint32_t)(((s & 1) * 2 + t) * 64);
-          const uint32_t td = tbase + kTmemD + (uint32_t)(((s & 1) * 2 + t) * 64);
-          for (int p = 0; p < a.parts; ++p) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              mma_f16(td + (uint32_t)(j * R / 8 * N), ta + 8 * j, bd + (uint64_t)((p * 8 + j) * (N * 32) / 16), idesc,
-                      (p > 0 || j % (8 / R) != 0) ? 1u : 0u);
-          }
-        }
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                         smem_u32(&B.done[s & 1]))
-                     : "memory");
-        B.issued = s;
-        // step s - 1's stage is free once its MMAs have read its activations
-        // (its weights and scales were read before they were issued)
-        if (s > 0 && s - 1 + a.stages < nsteps) {
-          if (!mbar_wait_bounded(&B.done[(s - 1) & 1], (uint32_t)(((s - 1) >> 1) & 1), a.wait_ns)) {
-            fail = true;
-            break;
-          }
-          stage(s - 1 + a.stages);
+          g0 = 0;
+          left = per;
         }
       }
     }
     fail = __any_sync(0xffffffffu, fail);
+  } else if (warp == kMmaWarp) {
+    const uint32_t leader = elect_one();
+    constexpr uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
+                               ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    // no-swizzle K-major descriptor: 128 bytes from a row's first 8 columns to
+    // its next 8, 256 from 8 rows to the next
+    const uint64_t bd0 = (uint64_t)(((smem_u32(smem) + (uint32_t)a.x_off) >> 4) & 0x3FFFu) |
+                         ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46);
+    int slot = 0, fslot = 0;  // the step's stage; the stage of the step two before and its phase
+    uint32_t fphase = 0;
+    for (int s = 0; s < nsteps; ++s) {
+      // step s - 2 had the same accumulators
+      if (!warp_wait(&B.ready[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns) ||
+          (s >= 2 && !warp_wait(&B.free[fslot], fphase, a.wait_ns))) {
+        fail = true;
+        break;
+      }
+      if (s >= 2 && ++fslot == a.stages) {
+        fslot = 0;
+        fphase ^= 1;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t bd = bd0 + (uint64_t)(slot * (a.stage_bytes >> 4));
+      const uint32_t ab = tbase + (uint32_t)((s & 1) * 128), db = ab + kTmemD;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j % (8 / R) == 0)
+            mma_f16<false>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+          else
+            mma_f16<true>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+        }
+      }
+      for (int p = 1; p < a.parts; ++p) {
+        const uint64_t bp = bd + (uint64_t)(p * 8 * N * 2);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            mma_f16<true>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bp + j * (N * 2), idesc, leader);
+      }
+      if (leader) {
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                         smem_u32(&B.done[s & 1]))
+                     : "memory");
+        B.issued = s;
+      }
+      __syncwarp();
+      if (++slot == a.stages) slot = 0;
+    }
   } else {
-    const int quarter = warp & 3, t = (warp >> 2) & 1, half = warp >> 3;
+    const int quarter = warp & 3, t = (warp >> 2) & 1, set = warp >> 3;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
-    const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-    float acc[CPT], sc[R], mn[R], nsc[R], nmn[R];
+    const uint32_t tw = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(t * 64);
+    float acc[CPT];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) acc[j] = 0.0f;
-    int ends = 0;  // tiles joined so far (phase of the joining barriers)
-    int tile = tile0, k = k0;  // position of the step being added
-    int uk = k0;               // column step being unpacked
+    const Unpack<BF16> unpack;
+    int ends = 0;              // tiles joined so far (phase of the joining barriers)
+    int tile = tile0, k = k0;  // position of the step being added, its stage and phase
+    int aslot = 0;
+    uint32_t aphase = 0;
+    int slot = set;            // stage and phase of the step being unpacked
+    uint32_t phase = 0;
 
     // adds step s's sums; at the end of a tile, or of this CTA's steps, writes
     auto add = [&](int s) -> bool {
-      if (__any_sync(0xffffffffu, !mbar_wait_bounded(&B.done[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns))) return false;
+      // (the stage has landed long since: that wait orders the scales' copies)
+      if (!warp_wait(&B.done[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns) ||
+          !warp_wait(&B.full[aslot], aphase, a.wait_ns))
+        return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t td = tbase + kTmemD + lanes + (uint32_t)(((s & 1) * 2 + t) * 64 + half * CPT);
+      const uint8_t* st = smem + (uint32_t)(aslot * a.stage_bytes);
+      const uint32_t td = tw + kTmemD + (uint32_t)((s & 1) * 128 + set * CPT);
       constexpr int C = CPT < 8 ? CPT : 8;
+      float sc[R];
 #pragma unroll
       for (int c = 0; c < CPT; c += C) {
-        uint32_t d[R][C];
+        uint32_t d[R][P][C];
 #pragma unroll
-        for (int r = 0; r < R; ++r) tmem_ld<C>(td + (uint32_t)(r * N + c), d[r]);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int p = 0; p < P; ++p) tmem_ld<C>(td + (uint32_t)(r * N + p * 2 * CPT + c), d[r][p]);
+        if (c == 0) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)  // (a short last step has fewer groups)
+            sc[r] = R == 1 || k * R + r < a.ngroups ? ld_scale(st + a.s_off, a.stype, r * kTile + row) : 0.0f;
+        }
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int j = 0; j < C; ++j) acc[c + j] = __fmaf_rn(sc[r], __uint_as_float(d[r][j]), acc[c + j]);
+          for (int j = 0; j < C; ++j) {
+            float v = __uint_as_float(d[r][0][j]);
+            if constexpr (FOLD) v = (__uint_as_float(d[r][2][j]) + __uint_as_float(d[r][1][j])) + v;
+            acc[c + j] = __fmaf_rn(sc[r], v, acc[c + j]);
+          }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       if (a.mins) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float* xs = a.xsum + ((size_t)k * R + r) * N + half * CPT;
+          if (R > 1 && k * R + r >= a.ngroups) break;
+          const float m = __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, r * kTile + row));
+          const float* xs = a.xsum + ((size_t)k * R + r) * N + set * CPT;
 #pragma unroll
-          for (int j = 0; j < CPT; ++j) acc[j] = __fmaf_rn(mn[r], xs[j], acc[j]);
+          for (int j = 0; j < CPT; ++j) acc[j] = __fmaf_rn(m, xs[j], acc[j]);
         }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.free[aslot]);
+      if (++aslot == a.stages) {
+        aslot = 0;
+        aphase ^= 1;
       }
       if (k + 1 < a.ksteps && s + 1 < nsteps) {
         ++k;
@@ -441,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int r = tile * kTile + row;
       bool write = true;
       if (first != 0 || k + 1 != a.ksteps) {
-        float* mine = a.part + ((size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * N + half * CPT) * kTile + row;
+        float* mine = a.part + ((size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * N + set * CPT) * kTile + row;
 #pragma unroll
         for (int j = 0; j < CPT; ++j) __stcg(mine + j * kTile, acc[j]);
         __threadfence();
@@ -449,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&B.joined);
         const uint32_t ph = (uint32_t)(ends & 1);
         if (warp == 0) {
-          if (__any_sync(0xffffffffu, !mbar_wait_bounded(&B.joined, ph, a.wait_ns))) return false;
+          if (!warp_wait(&B.joined, ph, a.wait_ns)) return false;
           if (lane == 0) {
             __threadfence();
             const int had = atomicAdd(a.count + tile, k + 1 - first);
@@ -457,8 +573,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             B.last = had + (k + 1 - first) == a.ksteps;
             mbar_arrive(&B.told);
           }
+          __syncwarp();
         }
-        if (__any_sync(0xffffffffu, !mbar_wait_bounded(&B.told, ph, a.wait_ns))) return false;
+        if (!warp_wait(&B.told, ph, a.wait_ns)) return false;
         ++ends;
         write = B.last != 0;
         if (write) {
@@ -471,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (;; ++c) {
             const int64_t b0 = a.steps * c / gridDim.x;
             if (b0 >= lo + a.ksteps) break;
-            const float* theirs = a.part + ((size_t)(2 * c + (b0 >= lo ? 0 : 1)) * N + half * CPT) * kTile + row;
+            const float* theirs = a.part + ((size_t)(2 * c + (b0 >= lo ? 0 : 1)) * N + set * CPT) * kTile + row;
 #pragma unroll
             for (int j = 0; j < CPT; ++j) acc[j] = __fadd_rn(acc[j], __ldcg(theirs + j * kTile));
             if (c + 1 == (int)gridDim.x) break;
@@ -481,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (write && r < a.rows) {
 #pragma unroll
         for (int j = 0; j < CPT; ++j)
-          if (half * CPT + j < a.nb) st_out(a.y, a.ytype, (int64_t)(half * CPT + j) * a.ldy + r, acc[j] * a.out_scale);
+          if (set * CPT + j < a.nb) st_out(a.y, a.ytype, (int64_t)(set * CPT + j) * a.ldy + r, acc[j] * a.out_scale);
       }
 #pragma unroll
       for (int j = 0; j < CPT; ++j) acc[j] = 0.0f;
@@ -490,50 +607,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
 
-    for (int s = 0; s < nsteps; ++s) {
-      const uint8_t* st = smem + (size_t)(s % a.stages) * a.stage_bytes;
-      if (__any_sync(0xffffffffu, !mbar_wait_bounded(&B.full[s % a.stages], (uint32_t)((s / a.stages) & 1), a.wait_ns))) {
+    // this set's steps s; each adds the two before it, in order
+    for (int s = set; !fail && s < nsteps; s += 2) {
+      if (!warp_wait(&B.full[slot], phase, a.wait_ns)) {
         fail = true;
         break;
       }
-      uint32_t raw[8];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        // 16-byte pieces of a 64-byte row lie where the 64-byte swizzle of
-        // the copy put them (free of bank conflicts)
-        const uint4 v = *reinterpret_cast<const uint4*>(st + row * 64 + (((2 * half + c) ^ ((row >> 1) & 3)) << 4));
-        raw[4 * c] = v.x;
-        raw[4 * c + 1] = v.y;
-        raw[4 * c + 2] = v.z;
-        raw[4 * c + 3] = v.w;
+      const uint8_t* st = smem + (uint32_t)(slot * a.stage_bytes) + row * 64;
+      slot += 2;
+      if (slot >= a.stages) {
+        slot -= a.stages;
+        phase ^= 1;
       }
-      const int g0 = (int)((int64_t)uk * kStep / a.group);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool in = g0 + r < a.ngroups;  // (a short last step has fewer groups)
-        nsc[r] = in ? ld_scale(st + a.s_off, a.stype, r * kTile + row) : 0.0f;
-        nmn[r] = in && a.mins ? __fmaf_rn(8.0f, nsc[r], ld_scale(st + a.m_off, a.stype, r * kTile + row)) : 0.0f;
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // 16-byte pieces of a 64-byte row lie where the 64-byte swizzle of
+          // the copy put them (free of bank conflicts)
+          const uint4 v = *reinterpret_cast<const uint4*>(st + (((2 * h + c) ^ ((row >> 1) & 3)) << 4));
+          unpack(v.x, o + 16 * c);
+          unpack(v.y, o + 16 * c + 4);
+          unpack(v.z, o + 16 * c + 8);
+          unpack(v.w, o + 16 * c + 12);
+        }
+        // (step s - 2 had the same operand buffer)
+        if (h == 0 && s >= 2 && !add(s - 2)) {
+          fail = true;
+          break;
+        }
+        tmem_st32(tw + (uint32_t)((s & 1) * 128 + h * 32), o);
       }
-      if (++uk == a.ksteps) uk = 0;
-      uint32_t o[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) unpack8<BF16>(raw[i], o + 4 * i);
-      tmem_st32(tbase + lanes + (uint32_t)(((s & 1) * 2 + t) * 64 + half * 32), o);
+      if (fail) break;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.ready[s & 1]);
-      if (s > 0 && !add(s - 1)) {
-        fail = true;
-        break;
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        sc[r] = nsc[r];
-        mn[r] = nmn[r];
-      }
+      if (s >= 1 && !add(s - 1)) fail = true;
     }
-    if (!fail && nsteps > 0 && !add(nsteps - 1)) fail = true;
+    // the last steps' sums: this set has added those before its last step
+    const int own = nsteps > set ? nsteps - 1 - ((nsteps - 1 - set) & 1) : -1;
+    for (int s = own < 0 ? 0 : own; !fail && s < nsteps; ++s) fail = !add(s);
   }
   if (fail) B.fail = 1;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -551,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == kWorkers)
+  if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(kTmemCols) : "memory");
 }
 
@@ -573,19 +688,22 @@ EncodeTiledFn encode_tiled() {
 
 
 template <bool BF16, int R>
-const void* kernel_of(int cpt) {
+const void* kernel_of(int cpt, bool fold) {
+  if constexpr (BF16) {
+    if (fold) return cpt == 1 ? (const void*)g4_kernel<true, 1, R, true> : (const void*)g4_kernel<true, 2, R, true>;
+  }
   switch (cpt) {
-    case 1: return (const void*)g4_kernel<BF16, 1, R>;
-    case 2: return (const void*)g4_kernel<BF16, 2, R>;
-    case 4: return (const void*)g4_kernel<BF16, 4, R>;
-    case 8: return (const void*)g4_kernel<BF16, 8, R>;
+    case 1: return (const void*)g4_kernel<BF16, 1, R, false>;
+    case 2: return (const void*)g4_kernel<BF16, 2, R, false>;
+    case 4: return (const void*)g4_kernel<BF16, 4, R, false>;
+    case 8: return (const void*)g4_kernel<BF16, 8, R, false>;
   }
   if constexpr (R <= 2) {
-    if (cpt == 16) return (const void*)g4_kernel<BF16, 16, R>;
+    if (cpt == 16) return (const void*)g4_kernel<BF16, 16, R, false>;
   }
   if constexpr (R == 1) {
-    if (cpt == 24) return (const void*)g4_kernel<BF16, 24, R>;
-    if (cpt == 32) return (const void*)g4_kernel<BF16, 32, R>;
+    if (cpt == 24) return (const void*)g4_kernel<BF16, 24, R, false>;
+    if (cpt == 32) return (const void*)g4_kernel<BF16, 32, R, false>;
   }
   return nullptr;
 }
@@ -628,7 +746,6 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   k.ldy = a.ldy;
   k.out_scale = a.xtype == NLS_DT_F16 ? 1.0f : 4096.0f;
   k.ksteps = p.ksteps;
-  k.parts = p.parts;
   k.steps = p.steps;
   k.wait_ns = a.wait_ns;
   k.status = a.status;
@@ -638,22 +755,24 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     k.nb = std::min(p.nmax, a.nb - b0);
     const int cpt = cols_per_thread(k.nb), n = mma_n(cpt);
     k.y = static_cast<uint8_t*>(a.y) + (size_t)b0 * a.ldy * yes;
+    const bool fold = folded(p.parts, k.nb);
+    k.parts = fold ? 1 : p.parts;  // MMA passes over the columns
     k.x_off = kRawBytes;
-    k.s_off = k.x_off + p.parts * n * kStep * 2;
+    k.s_off = k.x_off + k.parts * n * kStep * 2;
     k.m_off = k.s_off + p.regions * kTile * k.ssize;
     k.stage_bytes = (k.m_off + (a.mins ? p.regions * kTile * k.ssize : 0) + 1023) & ~1023;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Bars);
     k.stages = std::min(kMaxStages, room / k.stage_bytes);
     const size_t smem = (size_t)k.stages * k.stage_bytes + sizeof(Bars);
-    const void* kern = p.regions == 4 ? (bf16 ? kernel_of<true, 4>(cpt) : kernel_of<false, 4>(cpt))
-                       : p.regions == 2 ? (bf16 ? kernel_of<true, 2>(cpt) : kernel_of<false, 2>(cpt))
-                                        : (bf16 ? kernel_of<true, 1>(cpt) : kernel_of<false, 1>(cpt));
+    const void* kern = p.regions == 4 ? (bf16 ? kernel_of<true, 4>(cpt, fold) : kernel_of<false, 4>(cpt, fold))
+                       : p.regions == 2 ? (bf16 ? kernel_of<true, 2>(cpt, fold) : kernel_of<false, 2>(cpt, fold))
+                                        : (bf16 ? kernel_of<true, 1>(cpt, fold) : kernel_of<false, 1>(cpt, fold));
     if (!kern) return cudaErrorInvalidValue;
     const void* x = static_cast<const uint8_t*>(a.x) + (size_t)b0 * a.ldx * xes;
     with_type(a.xtype, [&](auto xv) {
       using X = decltype(xv);
       g4_layout_kernel<X><<<p.ksteps, 16 * n, 0, st>>>(static_cast<const X*>(x), a.ldx, k.nb, n, a.cols, p.parts,
-                                                       p.regions, ws, const_cast<float*>(k.xsum), k.count, p.tiles,
+                                                       fold ? 2 * cpt : 0, p.regions, ws, const_cast<float*>(k.xsum), k.count, p.tiles,
                                                        a.status, b0 == 0);
     });
     cudaError_t e = cudaGetLastError();
