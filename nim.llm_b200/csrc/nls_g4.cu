@@ -24,19 +24,21 @@
 // scale is then one register. The K order inside a word is the unpacking's
 // (0 4 1 5 2 6 3 7); the activations are laid out in that order once per call.
 //
-// Work: a tile is 256 weight rows (two MMAs of M = 128), a step 128 columns of
-// it. The steps of all tiles, in order, are dealt out evenly to the CTAs (one
+// Work: a tile is 256 weight rows (two MMAs of M = 128), a step 256 columns of
+// it: 128 bytes of a row, since the copy of a step costs the copy engine about
+// 4 cycles a row however short the row (64-byte rows held the kernel to 3.4
+// TB/s). The steps of all tiles, in order, are dealt out evenly to the CTAs (one
 // per SM), so an SM's load is within one step of every other's whatever the
 // shape; a tile that more than one CTA worked on is joined by the last of them
 // to finish, from partial sums in the workspace added in CTA order (the same
 // bits every time; no CTA waits for another).
-// One CTA: 16 worker warps in two sets, one that issues the copies (a ring of
-// stages: packed weights by tensor map, activations, scales) and one that
-// issues the MMAs. A set unpacks every other step (a thread 128 columns of its
-// row, so the waits, scales and bookkeeping of a step come once per 128
-// weights) and adds its half of the batch columns of every step's sums; while
-// one set unpacks, the other's MMAs run. Operands and accumulators have one
-// buffer per set in TMEM (2 x 128 and 2 x 128 columns).
+// One CTA, 26 warps: 16 unpack in two sets, each one half of a step's columns (a
+// thread 128 columns of its row); 8 add the halves' sums to their rows'; one
+// issues the copies (a ring of stages: packed weights by tensor map,
+// activations, scales) and one the MMAs. Roles only wait for one another
+// through mbarriers, and each runs as far ahead as its buffers let it: operands
+// have one buffer per set in TMEM (2 x 128 columns), accumulators as many as
+// fit in the other 256 columns.
 #include <cuda.h>
 
 #include <algorithm>
@@ -52,26 +54,27 @@ namespace nls {
 namespace {
 
 constexpr int kTile = 256;       // weight rows per tile
-constexpr int kStep = 128;       // columns per step
-constexpr int kWorkers = 16;     // warps, in two sets
-constexpr int kCopyWarp = kWorkers, kMmaWarp = kWorkers + 1;
-constexpr int kThreads = 32 * (kWorkers + 2);
+constexpr int kHalf = 128;       // columns per half of a step
+constexpr int kStep = 2 * kHalf;  // columns per step
+constexpr int kUnpackWarps = 16;  // two sets
+constexpr int kAddWarps = 8;
+constexpr int kCopyWarp = kUnpackWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemD = 256;  // A buffers below, accumulators from here on
 
-// batch rows per worker thread of a launch of nb (a set takes one half of
-// them), and the MMA's columns
-__host__ __device__ constexpr int cols_per_thread(int nb) {
-  return nb <= 2 ? 1 : nb <= 4 ? 2 : nb <= 8 ? 4 : nb <= 16 ? 8 : nb <= 32 ? 16 : nb <= 48 ? 24 : 32;
+// batch rows a launch is compiled for, and the MMA's columns. fp32 activations'
+// three parts are columns of their own up to 4 batch rows.
+__host__ __device__ constexpr int batch_of(int nb) {
+  return nb <= 1 ? 1 : nb <= 2 ? 2 : nb <= 4 ? 4 : nb <= 8 ? 8 : nb <= 16 ? 16 : nb <= 32 ? 32 : nb <= 48 ? 48 : 64;
 }
-__host__ __device__ constexpr int mma_n(int cpt) { return cpt <= 8 ? 16 : 2 * cpt; }
-// groups (scales) per step, and the most batch rows a launch takes with them:
-// each has 64 / regions accumulator columns of the 64 a tile half's buffer holds
-// fp32 activations' parts as columns of their own: up to 4 batch rows
+__host__ __device__ constexpr int mma_n(int nbt) { return nbt <= 16 ? 16 : nbt; }
 __host__ __device__ constexpr bool folded(int parts, int nb) { return parts == 3 && nb <= 4; }
+// groups (scales) per half step; its accumulators take regions x N columns per
+// tile half, 64 at most
 __host__ __device__ constexpr int regions_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
 
 struct Plan {
@@ -93,10 +96,11 @@ Plan plan_of(const G4Args& a, int sm_count) {
   p.grid = (int)std::min<int64_t>(sm_count, p.steps);
   p.parts = a.xtype == NLS_DT_F32 ? 3 : 1;
   p.regions = regions_of(a.group);
-  p.nmax = kMaxN / p.regions;
-  const int n = mma_n(cols_per_thread(std::min(a.nb, p.nmax)));
+  // (fp32's three parts: a stage of 64 rows would leave room for one stage only)
+  p.nmax = std::min(kMaxN / p.regions, p.parts == 3 ? 32 : kMaxN);
+  const int n = mma_n(batch_of(std::min(a.nb, p.nmax)));
   p.x_bytes = (size_t)p.ksteps * p.parts * n * (kStep * 2);
-  p.sum_bytes = a.mins ? (size_t)p.ksteps * p.regions * n * sizeof(float) : 0;
+  p.sum_bytes = a.mins ? (size_t)p.ksteps * 2 * p.regions * n * sizeof(float) : 0;
   p.part_bytes = (size_t)p.grid * 2 * n * kTile * sizeof(float);
   p.count_bytes = ((size_t)p.tiles * sizeof(int) + 15) & ~size_t(15);
   return p;
@@ -106,10 +110,11 @@ struct KernelArgs {
   const void* scales;
   const void* mins;
   int64_t s_ld;
-  int rows, cols, group, ngroups, ssize, stype;
+  int rows, group, ssize, stype;
+  int lines;            // lines of scales as the halves use them: of whole groups up to 128 wide, else per half
   int nb;
-  const uint8_t* x;     // laid-out activations, ksteps x parts x N x 256 bytes
-  const float* xsum;    // their sums [ksteps][regions][N]
+  const uint8_t* x;     // laid-out activations, per half step parts x N x 256 bytes
+  const float* xsum;    // their sums [half step][regions][N]
   float* part;          // partial tiles [2 * grid][N][256]
   int* count;           // steps joined so far, per tile
   void* y;
@@ -123,7 +128,7 @@ struct KernelArgs {
 };
 
 // ---- the activations' layout ------------------------------------------------
-// One block per step; a thread takes 8 columns of a batch row and writes them,
+// One block per half step; a thread takes 8 columns of a batch row and writes them,
 // permuted, as one 16-byte line of the operand (no-swizzle K-major: 8 rows x 16
 // bytes per core matrix, K step j of 16 columns at j * N * 32), for each part.
 // With minimums it also sums them per region (the 16 threads of a batch row
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
   for (int i = k * (int)blockDim.x + (int)threadIdx.x; i < tiles; i += (int)(gridDim.x * blockDim.x)) count[i] = 0;
   constexpr bool kF32 = std::is_same<X, float>::value;
   constexpr float kIn = std::is_same<X, __half>::value ? 1.0f : 0x1p-12f;
-  const int c0 = k * kStep + word * 8;
+  const int c0 = k * kHalf + word * 8;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.0f;
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
   constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
   // fold > 0: part p of batch row n is column p * fold + n (columns past the
   // parts are zeros: threads n >= fold write them)
-  uint8_t* dst = op + (size_t)k * (fold ? 1 : parts) * n_cols * (kStep * 2) + (size_t)(word >> 1) * (n_cols * 32) +
+  uint8_t* dst = op + (size_t)k * (fold ? 1 : parts) * n_cols * (kHalf * 2) + (size_t)(word >> 1) * (n_cols * 32) +
                  (word & 1) * 128;
   auto line = [&](int c) { return dst + (c >> 3) * 256 + (c & 7) * 16; };
   if (fold && n >= fold) {
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
       }
       w[j] = h[0] | (h[1] << 16);
     }
-    uint8_t* at = fold ? line(part * fold + n) : line(n) + (size_t)part * n_cols * (kStep * 2);
+    uint8_t* at = fold ? line(part * fold + n) : line(n) + (size_t)part * n_cols * (kHalf * 2);
     *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
@@ -320,50 +325,92 @@ __device__ __forceinline__ void st_out(void* y, int ytype, int64_t i, float v) {
   else reinterpret_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
 }
 
+constexpr int kMaxBuffers = 8;  // accumulator buffers
+
 struct Bars {
-  uint64_t full[kMaxStages];  // stage landed
-  uint64_t free[kMaxStages];  // every worker has added the step's sums (its MMAs are done, its scales read)
-  uint64_t ready[2];          // the set has stored its step's operand
-  uint64_t done[2];           // the step's MMAs have completed
-  uint64_t joined;            // every worker has written its partial sums
-  uint64_t told;              // whether this CTA is the tile's last
+  uint64_t full[kMaxStages];    // stage landed
+  uint64_t free[kMaxStages];    // the step's sums are added (its MMAs are done, its scales read)
+  uint64_t ready[2];            // the set has stored its half's operand
+  uint64_t done[kMaxBuffers];   // a half's MMAs have completed
+  uint64_t added[kMaxBuffers];  // its sums have been read
+  uint64_t joined;              // every adding warp has written its partial sums
+  uint64_t told;                // whether this CTA is the tile's last
   uint32_t tmem;
   int fail, staged, issued, last;
 };
 
+// barriers by their shared-memory address (32-bit arithmetic)
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (true) {
+    if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > limit_ns)) return false;
+  }
+}
 // a whole warp's bounded wait (the same answer in every lane)
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
-  if (limit_ns == 0) return false;
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return !__any_sync(0xffffffffu, !mbar_wait_bounded(bar, parity, limit_ns));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+  if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+  return warp_wait_slow(bar, parity, limit_ns);
 }
 
-// CPT: batch rows per thread. R: groups per step. FOLD: the three parts of fp32
-// activations are columns of their own (part p of batch row b in column
-// 2 CPT p + b), else further MMAs into the same columns.
-template <bool BF16, int CPT, int R, bool FOLD>
+// a position in a ring of n and the phase of its barriers there
+struct Ring {
+  int i;
+  uint32_t phase;
+  __device__ __forceinline__ void next(int n, int by = 1) {
+    i += by;
+    if (i >= n) {
+      i -= n;
+      phase ^= 1;
+    }
+  }
+};
+
+// NB: batch rows. R: groups per step. FOLD: the three parts of fp32 activations
+// are columns of their own (part p of batch row b in column NB p + b), else
+// further MMAs into the same columns.
+template <bool BF16, int NB, int R, bool FOLD>
 __global__ void __launch_bounds__(kThreads, 1)
     g4_kernel(const KernelArgs a, const __grid_constant__ CUtensorMap qmap) {
-  constexpr int N = mma_n(CPT);
+  constexpr int N = mma_n(NB);
   constexpr int P = FOLD ? 3 : 1;
-  static_assert(2 * CPT * P <= N && R * N <= 64, "columns");
+  constexpr int kBuffers = 128 / (R * N) < kMaxBuffers ? 128 / (R * N) : kMaxBuffers;
+  static_assert(NB * P <= N && R * N <= 64 && kBuffers >= 2, "columns");
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars& B = *reinterpret_cast<Bars*>(smem + (size_t)a.stages * a.stage_bytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t s0 = a.steps * blockIdx.x / gridDim.x, s1 = a.steps * (blockIdx.x + 1) / gridDim.x;
   const int nsteps = (int)(s1 - s0);
   const int tile0 = (int)(s0 / a.ksteps), k0 = (int)(s0 % a.ksteps);
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t full0 = smem_u32(B.full), free0 = smem_u32(B.free), ready0 = smem_u32(B.ready), done0 = smem_u32(B.done),
+                 added0 = smem_u32(B.added);
 
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&B.full[i], 1);
-      mbar_init(&B.free[i], kWorkers);
+      mbar_init(&B.free[i], kAddWarps);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&B.ready[i], kWorkers / 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.ready[i], kUnpackWarps / 2);
+    for (int i = 0; i < kMaxBuffers; ++i) {
       mbar_init(&B.done[i], 1);
+      mbar_init(&B.added[i], kAddWarps);
     }
-    mbar_init(&B.joined, kWorkers);
+    mbar_init(&B.joined, kAddWarps);
     mbar_init(&B.told, 1);
     B.fail = 0;
     B.staged = B.issued = -1;
@@ -382,51 +429,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the laid-out activations, their sums and the cleared counters are there
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  bool fail = false;
-  if (warp == kCopyWarp) {
+  // (a limit of 0 is a deadline already past: every role but the copies, whose
+  // first steps wait for nothing, gives up before its first wait)
+  bool fail = a.wait_ns == 0 && warp != kCopyWarp;
+  if (fail) {
+  } else if (warp == kCopyWarp) {
     if (lane == 0) {
       // position of the next step; its stage and the phase its last step left
-      // there; its group and, where groups are wider than a step, the steps
-      // left in it
-      int ltile = tile0, lk = k0, slot = 0;
-      uint32_t phase = 1;
-      const int per = R == 1 ? a.group / kStep : 1;
-      int g0 = R == 1 ? k0 / per : k0 * R, left = per - (R == 1 ? k0 % per : 0);
+      // there; where groups are at least as wide as a half, the next half's
+      // group and the halves left in it
+      int ltile = tile0, lk = k0;
+      Ring slot{0, 1};
+      const int per = R == 1 ? a.group / kHalf : 1;
+      int g1 = 2 * k0 / per, left = per - 2 * k0 % per;
       const uint32_t xb = (uint32_t)(a.parts * N * kStep * 2);
       for (int s = 0; s < nsteps; ++s) {
-        if (s >= a.stages && !mbar_wait_bounded(&B.free[slot], phase, a.wait_ns)) {
+        if (s >= a.stages && !mbar_wait_bounded(&B.free[slot.i], slot.phase, a.wait_ns)) {
           fail = true;
           break;
         }
-        uint8_t* st = smem + (size_t)slot * a.stage_bytes;
-        uint64_t* bar = &B.full[slot];
+        uint8_t* st = smem + (size_t)slot.i * a.stage_bytes;
+        uint64_t* bar = &B.full[slot.i];
         const int r0 = ltile * kTile;
         const uint32_t line = (uint32_t)(min(kTile, (a.rows - r0 + 7) & ~7) * a.ssize);
-        const int ng = min(R, a.ngroups - g0);
-        mbar_arrive_expect_tx(bar, kRawBytes + xb + (uint32_t)ng * line * (a.mins ? 2u : 1u));
+        const int n = min(2 * R, a.lines - 2 * R * lk);
+        mbar_arrive_expect_tx(bar, kRawBytes + xb + (uint32_t)n * line * (a.mins ? 2u : 1u));
         tma_load_2d(st, &qmap, lk * (kStep / 2), r0, bar);
         bulk_copy_g2s(st + a.x_off, a.x + (size_t)lk * xb, xb, bar);
-        for (int g = 0; g < ng; ++g) {
-          const size_t at = ((size_t)(g0 + g) * a.s_ld + r0) * a.ssize;
-          bulk_copy_g2s(st + a.s_off + g * kTile * a.ssize, static_cast<const uint8_t*>(a.scales) + at, line, bar);
+        for (int i = 0; i < n; ++i) {
+          int g = 2 * R * lk + i;
+          if (R == 1) {
+            g = g1;
+            if (--left == 0) {
+              left = per;
+              ++g1;
+            }
+          }
+          const size_t at = ((size_t)g * a.s_ld + r0) * a.ssize;
+          bulk_copy_g2s(st + a.s_off + i * kTile * a.ssize, static_cast<const uint8_t*>(a.scales) + at, line, bar);
           if (a.mins)
-            bulk_copy_g2s(st + a.m_off + g * kTile * a.ssize, static_cast<const uint8_t*>(a.mins) + at, line, bar);
+            bulk_copy_g2s(st + a.m_off + i * kTile * a.ssize, static_cast<const uint8_t*>(a.mins) + at, line, bar);
         }
         B.staged = s;
-        if (++slot == a.stages) {
-          slot = 0;
-          phase ^= 1;
-        }
-        if (R > 1) {
-          g0 += R;
-        } else if (--left == 0) {
-          left = per;
-          ++g0;
-        }
+        slot.next(a.stages);
         if (++lk == a.ksteps) {
           lk = 0;
           ++ltile;
-          g0 = 0;
+          g1 = 0;
           left = per;
         }
       }
@@ -438,144 +487,200 @@ __global__ void __launch_bounds__(kThreads, 1)
                                ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     // no-swizzle K-major descriptor: 128 bytes from a row's first 8 columns to
     // its next 8, 256 from 8 rows to the next
-    const uint64_t bd0 = (uint64_t)(((smem_u32(smem) + (uint32_t)a.x_off) >> 4) & 0x3FFFu) |
-                         ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46);
-    int slot = 0, fslot = 0;  // the step's stage; the stage of the step two before and its phase
-    uint32_t fphase = 0;
+    const uint64_t bd0 = (uint64_t)(((sbase + (uint32_t)a.x_off) >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) |
+                         ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46);
+    Ring slot{0, 0}, buf{0, 1};  // stage; accumulators, with the phase of their last use
+    for (int s = 0; s < nsteps && !fail; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!warp_wait(ready0 + (uint32_t)h * 8, (uint32_t)(s & 1), a.wait_ns) ||
+            (2 * s + h >= kBuffers && !warp_wait(added0 + (uint32_t)buf.i * 8, buf.phase, a.wait_ns))) {
+          fail = true;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t bd = bd0 + (uint64_t)(slot.i * (a.stage_bytes >> 4) + h * a.parts * (N * kHalf * 2 / 16));
+        const uint32_t ab = tbase + (uint32_t)(h * 128), db = tbase + kTmemD + (uint32_t)(buf.i * (2 * R * N));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j % (8 / R) == 0)
+              mma_f16<false>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+            else
+              mma_f16<true>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+          }
+        }
+        for (int p = 1; p < a.parts; ++p) {
+          const uint64_t bp = bd + (uint64_t)(p * 8 * N * 2);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              mma_f16<true>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bp + j * (N * 2), idesc, leader);
+        }
+        if (leader) {
+          asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                           done0 + (uint32_t)buf.i * 8)
+                       : "memory");
+          B.issued = 2 * s + h;
+        }
+        __syncwarp();
+        buf.next(kBuffers);
+      }
+      slot.next(a.stages);
+    }
+  } else if (warp < kUnpackWarps) {
+    const int quarter = warp & 3, t = (warp >> 2) & 1, set = warp >> 3;
+    const int row = t * 128 + quarter * 32 + lane;  // in the tile
+    const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(set * 128 + t * 64);
+    const uint32_t bar = ready0 + (uint32_t)set * 8;
+    // 16-byte pieces of a 128-byte row lie where the 128-byte swizzle of the
+    // copy put them (free of bank conflicts)
+    uint32_t at[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + (((4 * set + c) ^ (row & 7)) << 4));
+    const Unpack<BF16> unpack;
+    Ring slot{0, 0}, prev{set, 0};  // stage; accumulators of the step before's half
     for (int s = 0; s < nsteps; ++s) {
-      // step s - 2 had the same accumulators
-      if (!warp_wait(&B.ready[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns) ||
-          (s >= 2 && !warp_wait(&B.free[fslot], fphase, a.wait_ns))) {
+      if (!warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns)) {
         fail = true;
         break;
       }
-      if (s >= 2 && ++fslot == a.stages) {
-        fslot = 0;
-        fphase ^= 1;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t bd = bd0 + (uint64_t)(slot * (a.stage_bytes >> 4));
-      const uint32_t ab = tbase + (uint32_t)((s & 1) * 128), db = ab + kTmemD;
+      const uint32_t st = (uint32_t)(slot.i * a.stage_bytes);
+      slot.next(a.stages);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j % (8 / R) == 0)
-            mma_f16<false>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
-          else
-            mma_f16<true>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(at[2 * h + c] + st)
+                       : "memory");
+#pragma unroll
+          for (int i = 0; i < 4; ++i) unpack(v[i], o + 16 * c + 4 * i);
         }
+        // the step before had the same operand buffer
+        if (h == 0 && s >= 1) {
+          if (!warp_wait(done0 + (uint32_t)prev.i * 8, prev.phase, a.wait_ns)) {
+            fail = true;
+            break;
+          }
+          prev.next(kBuffers, 2);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        tmem_st32(ta + h * 32, o);
       }
-      for (int p = 1; p < a.parts; ++p) {
-        const uint64_t bp = bd + (uint64_t)(p * 8 * N * 2);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            mma_f16<true>(db + t * 64 + j * R / 8 * N, ab + t * 64 + 8 * j, bp + j * (N * 2), idesc, leader);
-      }
-      if (leader) {
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                         smem_u32(&B.done[s & 1]))
-                     : "memory");
-        B.issued = s;
-      }
+      if (fail) break;
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (++slot == a.stages) slot = 0;
+      if (lane == 0) arrive(bar);
     }
   } else {
-    const int quarter = warp & 3, t = (warp >> 2) & 1, set = warp >> 3;
+    const int aw = warp - kUnpackWarps, quarter = aw & 3, t = aw >> 2;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
-    const uint32_t tw = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(t * 64);
-    float acc[CPT];
+    const uint32_t td = tbase + ((uint32_t)(32 * quarter) << 16) + kTmemD + (uint32_t)(t * R * N);
+    float acc[NB];
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) acc[j] = 0.0f;
-    const Unpack<BF16> unpack;
+    for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
     int ends = 0;              // tiles joined so far (phase of the joining barriers)
-    int tile = tile0, k = k0;  // position of the step being added, its stage and phase
-    int aslot = 0;
-    uint32_t aphase = 0;
-    int slot = set;            // stage and phase of the step being unpacked
-    uint32_t phase = 0;
-
-    // adds step s's sums; at the end of a tile, or of this CTA's steps, writes
-    auto add = [&](int s) -> bool {
-      // (the stage has landed long since: that wait orders the scales' copies)
-      if (!warp_wait(&B.done[s & 1], (uint32_t)((s >> 1) & 1), a.wait_ns) ||
-          !warp_wait(&B.full[aslot], aphase, a.wait_ns))
-        return false;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint8_t* st = smem + (uint32_t)(aslot * a.stage_bytes);
-      const uint32_t td = tw + kTmemD + (uint32_t)((s & 1) * 128 + set * CPT);
-      constexpr int C = CPT < 8 ? CPT : 8;
-      float sc[R];
-#pragma unroll
-      for (int c = 0; c < CPT; c += C) {
-        uint32_t d[R][P][C];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int p = 0; p < P; ++p) tmem_ld<C>(td + (uint32_t)(r * N + p * 2 * CPT + c), d[r][p]);
-        if (c == 0) {
-#pragma unroll
-          for (int r = 0; r < R; ++r)  // (a short last step has fewer groups)
-            sc[r] = R == 1 || k * R + r < a.ngroups ? ld_scale(st + a.s_off, a.stype, r * kTile + row) : 0.0f;
+    int tile = tile0, k = k0;  // position of the step
+    Ring slot{0, 0}, buf{0, 0};
+    for (int s = 0; s < nsteps; ++s) {
+      const uint8_t* st = smem + (uint32_t)(slot.i * a.stage_bytes);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        // (the stage has landed long since: that wait orders the scales' copies)
+        if (!warp_wait(done0 + (uint32_t)buf.i * 8, buf.phase, a.wait_ns) ||
+            (h == 0 && !warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns))) {
+          fail = true;
+          break;
         }
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d0 = td + (uint32_t)(buf.i * (2 * R * N));
+        const int l0 = (2 * k + h) * R;  // the half's first line of scales
+        constexpr int C = NB < 8 ? NB : 8;
+        float sc[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int c = 0; c < NB; c += C) {
+          uint32_t d[R][P][C];
 #pragma unroll
-          for (int j = 0; j < C; ++j) {
-            float v = __uint_as_float(d[r][0][j]);
-            if constexpr (FOLD) v = (__uint_as_float(d[r][2][j]) + __uint_as_float(d[r][1][j])) + v;
-            acc[c + j] = __fmaf_rn(sc[r], v, acc[c + j]);
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int p = 0; p < P; ++p) tmem_ld<C>(d0 + (uint32_t)(r * N + p * NB + c), d[r][p]);
+          if (c == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)  // (the last step may have fewer)
+              sc[r] = l0 + r < a.lines ? ld_scale(st + a.s_off, a.stype, (h * R + r) * kTile + row) : 0.0f;
           }
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      if (a.mins) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          if (R > 1 && k * R + r >= a.ngroups) break;
-          const float m = __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, r * kTile + row));
-          const float* xs = a.xsum + ((size_t)k * R + r) * N + set * CPT;
+          for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int j = 0; j < CPT; ++j) acc[j] = __fmaf_rn(m, xs[j], acc[j]);
+            for (int j = 0; j < C; ++j) {
+              float v = __uint_as_float(d[r][0][j]);
+              if constexpr (FOLD) v = (__uint_as_float(d[r][2][j]) + __uint_as_float(d[r][1][j])) + v;
+              acc[c + j] = __fmaf_rn(sc[r], v, acc[c + j]);
+            }
         }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (a.mins) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (l0 + r >= a.lines) break;
+            const float m = __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, (h * R + r) * kTile + row));
+            const float* xs = a.xsum + (size_t)(l0 + r) * N;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(m, xs[j], acc[j]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          arrive(added0 + (uint32_t)buf.i * 8);
+          if (h == 1) arrive(free0 + (uint32_t)slot.i * 8);
+        }
+        buf.next(kBuffers);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.free[aslot]);
-      if (++aslot == a.stages) {
-        aslot = 0;
-        aphase ^= 1;
-      }
+      if (fail) break;
+      slot.next(a.stages);
       if (k + 1 < a.ksteps && s + 1 < nsteps) {
         ++k;
-        return true;
+        continue;
       }
-      // the tile's steps of this CTA were [first, k]
+      // the end of a tile, or of this CTA's steps; the tile's steps of this
+      // CTA were [first, k]
       const int first = tile == tile0 ? k0 : 0;
       const int r = tile * kTile + row;
       bool write = true;
       if (first != 0 || k + 1 != a.ksteps) {
-        float* mine = a.part + ((size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * N + set * CPT) * kTile + row;
+        float* mine = a.part + (size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * N * kTile + row;
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) __stcg(mine + j * kTile, acc[j]);
+        for (int j = 0; j < NB; ++j) __stcg(mine + j * kTile, acc[j]);
         __threadfence();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.joined);
+        if (lane == 0) arrive(smem_u32(&B.joined));
         const uint32_t ph = (uint32_t)(ends & 1);
-        if (warp == 0) {
-          if (!warp_wait(&B.joined, ph, a.wait_ns)) return false;
+        if (aw == 0) {
+          if (!warp_wait(smem_u32(&B.joined), ph, a.wait_ns)) {
+            fail = true;
+            break;
+          }
           if (lane == 0) {
             __threadfence();
             const int had = atomicAdd(a.count + tile, k + 1 - first);
             __threadfence();
             B.last = had + (k + 1 - first) == a.ksteps;
-            mbar_arrive(&B.told);
+            arrive(smem_u32(&B.told));
           }
           __syncwarp();
         }
-        if (!warp_wait(&B.told, ph, a.wait_ns)) return false;
+        if (!warp_wait(smem_u32(&B.told), ph, a.wait_ns)) {
+          fail = true;
+          break;
+        }
         ++ends;
         write = B.last != 0;
         if (write) {
@@ -584,71 +689,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t lo = (int64_t)tile * a.ksteps;
           int c = (int)(((lo + 1) * gridDim.x - 1) / a.steps);
 #pragma unroll
-          for (int j = 0; j < CPT; ++j) acc[j] = 0.0f;
+          for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
           for (;; ++c) {
             const int64_t b0 = a.steps * c / gridDim.x;
             if (b0 >= lo + a.ksteps) break;
-            const float* theirs = a.part + ((size_t)(2 * c + (b0 >= lo ? 0 : 1)) * N + set * CPT) * kTile + row;
+            const float* theirs = a.part + (size_t)(2 * c + (b0 >= lo ? 0 : 1)) * N * kTile + row;
 #pragma unroll
-            for (int j = 0; j < CPT; ++j) acc[j] = __fadd_rn(acc[j], __ldcg(theirs + j * kTile));
+            for (int j = 0; j < NB; ++j) acc[j] = __fadd_rn(acc[j], __ldcg(theirs + j * kTile));
             if (c + 1 == (int)gridDim.x) break;
           }
         }
       }
       if (write && r < a.rows) {
 #pragma unroll
-        for (int j = 0; j < CPT; ++j)
-          if (set * CPT + j < a.nb) st_out(a.y, a.ytype, (int64_t)(set * CPT + j) * a.ldy + r, acc[j] * a.out_scale);
+        for (int j = 0; j < NB; ++j)
+          if (j < a.nb) st_out(a.y, a.ytype, (int64_t)j * a.ldy + r, acc[j] * a.out_scale);
       }
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
       ++tile;
       k = 0;
-      return true;
-    };
-
-    // this set's steps s; each adds the two before it, in order
-    for (int s = set; !fail && s < nsteps; s += 2) {
-      if (!warp_wait(&B.full[slot], phase, a.wait_ns)) {
-        fail = true;
-        break;
-      }
-      const uint8_t* st = smem + (uint32_t)(slot * a.stage_bytes) + row * 64;
-      slot += 2;
-      if (slot >= a.stages) {
-        slot -= a.stages;
-        phase ^= 1;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t o[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          // 16-byte pieces of a 64-byte row lie where the 64-byte swizzle of
-          // the copy put them (free of bank conflicts)
-          const uint4 v = *reinterpret_cast<const uint4*>(st + (((2 * h + c) ^ ((row >> 1) & 3)) << 4));
-          unpack(v.x, o + 16 * c);
-          unpack(v.y, o + 16 * c + 4);
-          unpack(v.z, o + 16 * c + 8);
-          unpack(v.w, o + 16 * c + 12);
-        }
-        // (step s - 2 had the same operand buffer)
-        if (h == 0 && s >= 2 && !add(s - 2)) {
-          fail = true;
-          break;
-        }
-        tmem_st32(tw + (uint32_t)((s & 1) * 128 + h * 32), o);
-      }
-      if (fail) break;
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.ready[s & 1]);
-      if (s >= 1 && !add(s - 1)) fail = true;
     }
-    // the last steps' sums: this set has added those before its last step
-    const int own = nsteps > set ? nsteps - 1 - ((nsteps - 1 - set) & 1) : -1;
-    for (int s = own < 0 ? 0 : own; !fail && s < nsteps; ++s) fail = !add(s);
   }
   if (fail) B.fail = 1;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -660,8 +721,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (under the default limit: they are real)
       for (int s = max(0, B.staged - a.stages + 1); s <= B.staged; ++s)
         (void)mbar_wait_bounded(&B.full[s % a.stages], (uint32_t)((s / a.stages) & 1));
-      for (int s = max(0, B.issued - 1); s <= B.issued; ++s)
-        (void)mbar_wait_bounded(&B.done[s & 1], (uint32_t)((s >> 1) & 1));
+      for (int s = max(0, B.issued - kBuffers + 1); s <= B.issued; ++s)
+        (void)mbar_wait_bounded(&B.done[s % kBuffers], (uint32_t)((s / kBuffers) & 1));
     }
     __syncthreads();
   }
@@ -688,22 +749,25 @@ EncodeTiledFn encode_tiled() {
 
 
 template <bool BF16, int R>
-const void* kernel_of(int cpt, bool fold) {
+const void* kernel_of(int nbt, bool fold) {
   if constexpr (BF16) {
-    if (fold) return cpt == 1 ? (const void*)g4_kernel<true, 1, R, true> : (const void*)g4_kernel<true, 2, R, true>;
+    if (fold)
+      return nbt == 1 ? (const void*)g4_kernel<true, 1, R, true>
+             : nbt == 2 ? (const void*)g4_kernel<true, 2, R, true> : (const void*)g4_kernel<true, 4, R, true>;
   }
-  switch (cpt) {
+  switch (nbt) {
     case 1: return (const void*)g4_kernel<BF16, 1, R, false>;
     case 2: return (const void*)g4_kernel<BF16, 2, R, false>;
     case 4: return (const void*)g4_kernel<BF16, 4, R, false>;
     case 8: return (const void*)g4_kernel<BF16, 8, R, false>;
+    case 16: return (const void*)g4_kernel<BF16, 16, R, false>;
   }
   if constexpr (R <= 2) {
-    if (cpt == 16) return (const void*)g4_kernel<BF16, 16, R, false>;
+    if (nbt == 32) return (const void*)g4_kernel<BF16, 32, R, false>;
   }
   if constexpr (R == 1) {
-    if (cpt == 24) return (const void*)g4_kernel<BF16, 24, R, false>;
-    if (cpt == 32) return (const void*)g4_kernel<BF16, 32, R, false>;
+    if (nbt == 48) return (const void*)g4_kernel<BF16, 48, R, false>;
+    if (nbt == 64) return (const void*)g4_kernel<BF16, 64, R, false>;
   }
   return nullptr;
 }
@@ -724,7 +788,7 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   const cuuint32_t box[2] = {kStep / 2, kTile};
   const cuuint32_t ones[2] = {1, 1};
   if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a.q), dims, strides, box, ones,
-          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
 
@@ -733,9 +797,8 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   k.mins = a.mins;
   k.s_ld = a.s_ld;
   k.rows = a.rows;
-  k.cols = a.cols;
   k.group = a.group;
-  k.ngroups = (a.cols + a.group - 1) / a.group;
+  k.lines = (a.cols + std::min(a.group, kHalf) - 1) / std::min(a.group, kHalf);
   k.stype = a.stype;
   k.ssize = (int)dt_size(a.stype);
   k.x = ws;
@@ -753,26 +816,26 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   const size_t xes = dt_size(a.xtype), yes = dt_size(a.ytype);
   for (int b0 = 0; b0 < a.nb; b0 += p.nmax) {
     k.nb = std::min(p.nmax, a.nb - b0);
-    const int cpt = cols_per_thread(k.nb), n = mma_n(cpt);
+    const int nbt = batch_of(k.nb), n = mma_n(nbt);
     k.y = static_cast<uint8_t*>(a.y) + (size_t)b0 * a.ldy * yes;
     const bool fold = folded(p.parts, k.nb);
     k.parts = fold ? 1 : p.parts;  // MMA passes over the columns
     k.x_off = kRawBytes;
     k.s_off = k.x_off + k.parts * n * kStep * 2;
-    k.m_off = k.s_off + p.regions * kTile * k.ssize;
-    k.stage_bytes = (k.m_off + (a.mins ? p.regions * kTile * k.ssize : 0) + 1023) & ~1023;
+    k.m_off = k.s_off + 2 * p.regions * kTile * k.ssize;
+    k.stage_bytes = (k.m_off + (a.mins ? 2 * p.regions * kTile * k.ssize : 0) + 1023) & ~1023;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Bars);
     k.stages = std::min(kMaxStages, room / k.stage_bytes);
     const size_t smem = (size_t)k.stages * k.stage_bytes + sizeof(Bars);
-    const void* kern = p.regions == 4 ? (bf16 ? kernel_of<true, 4>(cpt, fold) : kernel_of<false, 4>(cpt, fold))
-                       : p.regions == 2 ? (bf16 ? kernel_of<true, 2>(cpt, fold) : kernel_of<false, 2>(cpt, fold))
-                                        : (bf16 ? kernel_of<true, 1>(cpt, fold) : kernel_of<false, 1>(cpt, fold));
+    const void* kern = p.regions == 4 ? (bf16 ? kernel_of<true, 4>(nbt, fold) : kernel_of<false, 4>(nbt, fold))
+                       : p.regions == 2 ? (bf16 ? kernel_of<true, 2>(nbt, fold) : kernel_of<false, 2>(nbt, fold))
+                                        : (bf16 ? kernel_of<true, 1>(nbt, fold) : kernel_of<false, 1>(nbt, fold));
     if (!kern) return cudaErrorInvalidValue;
     const void* x = static_cast<const uint8_t*>(a.x) + (size_t)b0 * a.ldx * xes;
     with_type(a.xtype, [&](auto xv) {
       using X = decltype(xv);
-      g4_layout_kernel<X><<<p.ksteps, 16 * n, 0, st>>>(static_cast<const X*>(x), a.ldx, k.nb, n, a.cols, p.parts,
-                                                       fold ? 2 * cpt : 0, p.regions, ws, const_cast<float*>(k.xsum), k.count, p.tiles,
+      g4_layout_kernel<X><<<2 * p.ksteps, 16 * n, 0, st>>>(static_cast<const X*>(x), a.ldx, k.nb, n, a.cols, p.parts,
+                                                       fold ? nbt : 0, p.regions, ws, const_cast<float*>(k.xsum), k.count, p.tiles,
                                                        a.status, b0 == 0);
     });
     cudaError_t e = cudaGetLastError();
