@@ -5,24 +5,34 @@
 // With q' = q - 8 and, where there are minimums, m' = m + 8 s:
 //   y[b][r] = sum_g ( s[g][r] * sum_{c in g} q'[r][c] x[b][c]
 //                     + m'[g][r] * sum_{c in g} x[b][c] )
-// q' is exact in fp16 and bfloat16, so tcgen05.mma kind::f16 forms the inner
-// sums from exact products with fp32 accumulation, and the scales stay in fp32
-// outside them: no weight is rounded. fp32 activations are split into three
-// bfloat16 parts that hold all 24 bits, multiplied one after the other into
-// the same accumulator. fp32 and bfloat16 activations enter as x 2^-12, and
-// the result is multiplied by 2^12: 128 products with q' reach 2^10 times the
-// largest activation, which would pass fp32's range before the scales bring it
-// down.
+// The inner sums are formed by the tensor cores without rounding a weight, the
+// scales stay outside them in fp32. Two ways:
+//  * Integers (few batch rows). The activations of a row's 128 columns are
+//    fixed-point numbers X 2^-e of 31 bits (the largest has 30, so what is cut
+//    off is 2^-31 of it), split into four signed bytes, which are four columns
+//    of a tcgen05.mma kind::i8 against the nibbles themselves as unsigned
+//    bytes: every product and sum is exact. 8 sum(X) is taken off afterwards,
+//    in integers, and the four sums joined in fp32. Two or three logical
+//    operations unpack 8 weights.
+//  * Floating point (more batch rows: one column each instead of four). q' is
+//    exact in fp16 and bfloat16; kind::f16 sums exact products in fp32. fp32
+//    activations are split into three bfloat16 parts that hold all 24 bits,
+//    multiplied one after the other into the same accumulator. fp32 and
+//    bfloat16 activations enter as x 2^-12 and the result is multiplied by
+//    2^12: 128 products with q' reach 2^10 times the largest activation, which
+//    would pass fp32's range before the scales bring it down.
 //
 // What bounds it: at a few batch rows the weights' bytes (half a byte per
 // weight); turning them into operands is the work per byte. So the A operand
 // never touches shared memory: a thread owns a weight row, reads its packed
-// bytes from the staged tile, turns a 32-bit word into four packed pairs
-// (4 logical operations, 1-3 shifts and 4 packed fp16/bf16 operations per 8
-// weights) and stores them to tensor memory (tcgen05.st), from where the MMA
-// reads A; the sums come back to the same thread (tcgen05.ld), whose row's
-// scale is then one register. The K order inside a word is the unpacking's
-// (0 4 1 5 2 6 3 7); the activations are laid out in that order once per call.
+// bytes from the staged tile, unpacks them in registers and stores them to
+// tensor memory (tcgen05.st), from where the MMA reads A; the sums come back to
+// a thread of the same row (tcgen05.ld), whose scale is one register. The K
+// order inside a word is the unpacking's; the activations are laid out in that
+// order once per call. Unpacking to 16 bits (4 logical operations, 1-3 shifts
+// and 4 packed subtractions per 8 weights, and 4 bytes per packed byte into
+// tensor memory) holds the floating-point way to 60 % of the rate of the
+// integer one at one row.
 //
 // Work: a tile is 256 weight rows (two MMAs of M = 128), a step 256 columns of
 // it: 128 bytes of a row, since the copy of a step costs the copy engine about
@@ -62,46 +72,76 @@ constexpr int kCopyWarp = kUnpackWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
-constexpr int kMaxN = 64;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kTmemD = 256;  // A buffers below, accumulators from here on
 
-// batch rows a launch is compiled for, and the MMA's columns. fp32 activations'
-// three parts are columns of their own up to 4 batch rows.
-__host__ __device__ constexpr int batch_of(int nb) {
-  return nb <= 1 ? 1 : nb <= 2 ? 2 : nb <= 4 ? 4 : nb <= 8 ? 8 : nb <= 16 ? 16 : nb <= 32 ? 32 : nb <= 48 ? 48 : 64;
-}
-__host__ __device__ constexpr int mma_n(int nbt) { return nbt <= 16 ? 16 : nbt; }
-__host__ __device__ constexpr bool folded(int parts, int nb) { return parts == 3 && nb <= 4; }
-// groups (scales) per half step; its accumulators take regions x N columns per
-// tile half, 64 at most
+enum class Op { kI8, kF16, kBF16 };
+// Tensor memory: a half step's operand takes 32 (bytes) or 64 columns per tile
+// half, two tile halves in each set's buffer; the rest are accumulators
+__host__ __device__ constexpr int a_cols(Op op) { return op == Op::kI8 ? 32 : 64; }
+__host__ __device__ constexpr int acc_cols(Op op) { return (int)kTmemCols - 4 * a_cols(op); }
+
+// groups (scales) per half step
 __host__ __device__ constexpr int regions_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
+// batch rows a launch is compiled for, and the MMA's columns
+__host__ __device__ constexpr int batch_of(Op op, int nb) {
+  if (op == Op::kI8) return nb <= 1 ? 1 : nb <= 2 ? 2 : nb <= 4 ? 4 : nb <= 8 ? 8 : nb <= 12 ? 12 : 16;
+  return nb <= 8 ? 8 : nb <= 16 ? 16 : nb <= 32 ? 32 : nb <= 48 ? 48 : 64;
+}
+__host__ __device__ constexpr int mma_n(Op op, int nbt) {
+  return op == Op::kI8 ? (nbt <= 4 ? 16 : 4 * nbt) : (nbt <= 16 ? 16 : nbt);
+}
+// The most batch rows the integer way takes: two buffers of accumulators have
+// to fit in tensor memory (96 columns per tile half and buffer).
+__host__ __device__ constexpr int i8_rows(int regions) { return regions == 4 ? 4 : regions == 2 ? 12 : 16; }
+// bytes of a half step's laid-out activations: bytes (and per region and batch
+// row four words for the joining), or 16-bit parts
+__host__ __device__ constexpr int x_half(Op op, int nbt, int regions, int parts) {
+  return op == Op::kI8 ? mma_n(op, nbt) * kHalf + regions * nbt * 16 : parts * mma_n(op, nbt) * kHalf * 2;
+}
+
+// How a launch of nb batch rows goes.
+struct Way {
+  Op op;
+  int nb, nbt, n, parts;
+};
+
+Way way_of(const G4Args& a, int left) {
+  Way w;
+  const int regions = regions_of(a.group);
+  w.op = left <= i8_rows(regions) ? Op::kI8 : a.xtype == NLS_DT_F16 ? Op::kF16 : Op::kBF16;
+  w.parts = w.op != Op::kI8 && a.xtype == NLS_DT_F32 ? 3 : 1;
+  // regions x N columns: 64 per tile half and buffer. (fp32's three parts: a
+  // stage of 64 rows would leave room for one stage only)
+  w.nb = w.op == Op::kI8 ? left : std::min(left, std::min(64 / regions, w.parts == 3 ? 32 : 64));
+  w.nbt = batch_of(w.op, w.nb);
+  w.n = mma_n(w.op, w.nbt);
+  return w;
+}
 
 struct Plan {
-  int ksteps, tiles, grid;
-  int64_t steps;                 // tiles * ksteps
-  int parts;                     // bfloat16 parts of an activation: 3 for fp32
-  int regions;
-  int nmax;                      // batch rows per launch
+  int ksteps, tiles, grid, regions;
+  int64_t steps;  // tiles * ksteps
   // workspace
   size_t x_bytes, sum_bytes, part_bytes, count_bytes;
   size_t total() const { return x_bytes + sum_bytes + part_bytes + count_bytes; }
 };
 
 Plan plan_of(const G4Args& a, int sm_count) {
-  Plan p;
+  Plan p{};
   p.ksteps = (a.cols + kStep - 1) / kStep;
   p.tiles = (a.rows + kTile - 1) / kTile;
   p.steps = (int64_t)p.tiles * p.ksteps;
   p.grid = (int)std::min<int64_t>(sm_count, p.steps);
-  p.parts = a.xtype == NLS_DT_F32 ? 3 : 1;
   p.regions = regions_of(a.group);
-  // (fp32's three parts: a stage of 64 rows would leave room for one stage only)
-  p.nmax = std::min(kMaxN / p.regions, p.parts == 3 ? 32 : kMaxN);
-  const int n = mma_n(batch_of(std::min(a.nb, p.nmax)));
-  p.x_bytes = (size_t)p.ksteps * p.parts * n * (kStep * 2);
-  p.sum_bytes = a.mins ? (size_t)p.ksteps * 2 * p.regions * n * sizeof(float) : 0;
-  p.part_bytes = (size_t)p.grid * 2 * n * kTile * sizeof(float);
+  for (int b0 = 0; b0 < a.nb;) {
+    const Way w = way_of(a, a.nb - b0);
+    const size_t halves = (size_t)p.ksteps * 2;
+    p.x_bytes = std::max(p.x_bytes, (halves * x_half(w.op, w.nbt, p.regions, w.parts) + 255) & ~size_t(255));
+    if (a.mins && w.op != Op::kI8) p.sum_bytes = std::max(p.sum_bytes, halves * p.regions * w.n * sizeof(float));
+    p.part_bytes = std::max(p.part_bytes, (size_t)p.grid * 2 * w.nbt * kTile * sizeof(float));
+    b0 += w.nb;
+    if (a.nb - b0 > 2 * 64) b0 = a.nb - 64 - (a.nb - b0) % 64;  // (passes in between are all alike)
+  }
   p.count_bytes = ((size_t)p.tiles * sizeof(int) + 15) & ~size_t(15);
   return p;
 }
@@ -113,9 +153,9 @@ struct KernelArgs {
   int rows, group, ssize, stype;
   int lines;            // lines of scales as the halves use them: of whole groups up to 128 wide, else per half
   int nb;
-  const uint8_t* x;     // laid-out activations, per half step parts x N x 256 bytes
-  const float* xsum;    // their sums [half step][regions][N]
-  float* part;          // partial tiles [2 * grid][N][256]
+  const uint8_t* x;     // laid-out activations, x_half bytes per half step
+  const float* xsum;    // their sums [half step][regions][N] (floating point with minimums)
+  float* part;          // partial tiles [2 * grid][NB][256]
   int* count;           // steps joined so far, per tile
   void* y;
   int ytype;
@@ -128,41 +168,120 @@ struct KernelArgs {
 };
 
 // ---- the activations' layout ------------------------------------------------
-// One block per half step; a thread takes 8 columns of a batch row and writes them,
+
+// eight activations of a batch row as fp32 (past the matrix: zeros; columns come
+// in whole 32)
+template <class X>
+__device__ __forceinline__ void load8(const X* x, int64_t ldx, int nb, int cols, int n, int c0, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  if (n >= nb || c0 >= cols) return;
+  const X* p = x + (int64_t)n * ldx + c0;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    X t[8];
+#pragma unroll
+    for (int e = 0; e < (int)(8 * sizeof(X) / 16); ++e) reinterpret_cast<uint4*>(t)[e] = reinterpret_cast<const uint4*>(p)[e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32(t[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32(p[e]);
+  }
+}
+
+__device__ __forceinline__ void clear_counts(int* count, int tiles, int* status, int clear_status) {
+  const int i0 = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+  if (i0 == 0 && clear_status) *status = NLS_OK;
+  for (int i = i0; i < tiles; i += (int)(gridDim.x * blockDim.x)) count[i] = 0;
+}
+
+// The integer way. One block per half step; the 16 threads of a batch row take 8
+// columns each. Their largest magnitude gives the row's exponent there: X =
+// x 2^e with |X| < 2^30 is exact but for the rounding to a whole number; its
+// four bytes p0 2^24 + p1 2^16 + p2 2^8 + p3, each -128 .. 127, are columns 4 n
+// .. 4 n + 3 of the operand (no-swizzle K-major: 8 rows x 16 bytes per core
+// matrix, K step j of 32 columns at j * N * 32). Behind the operand, per
+// region and batch row: 8 (sum p0 2^8 + sum p1), 8 (sum p2 2^8 + sum p3), 2^-e
+// and sum X. A row with an infinity or a NaN has NaN for 2^-e. (The exponent
+// stops at 2^-96: 2^-e stays a normal number; what that loses is below 2^-125.)
+template <class X>
+__global__ void __launch_bounds__(512) g4_bytes_kernel(const X* x, int64_t ldx, int nb, int nbt, int n_cols, int cols,
+                                                       int regions, uint8_t* op, int half_bytes, int* count, int tiles,
+                                                       int* status, int clear_status) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  clear_counts(count, tiles, status, clear_status);
+  const int k = blockIdx.x, n = threadIdx.x >> 4, word = threadIdx.x & 15;
+  float v[8];
+  load8(x, ldx, nb, cols, n, k * kHalf + word * 8, v);
+  float top = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top = fmaxf(top, fabsf(v[e]));
+    bad |= !isfinite(v[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+  }
+  // top < 2^(E + 1), E the exponent field's: X below 2^30
+  const int E = max((int)(__float_as_uint(top) >> 23) - 127, -96);
+  const double up = __longlong_as_double((long long)(29 - E + 1023) << 52);
+  int sum[4] = {0, 0, 0, 0};
+  uint32_t lo[4] = {0u, 0u, 0u, 0u}, hi[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    int f = bad ? 0 : __double2int_rn((double)v[e] * up);
+#pragma unroll
+    for (int p = 3; p >= 0; --p) {
+      const int d = (int)(int8_t)(f & 0xFF);
+      f = (f - d) >> 8;
+      sum[p] += d;
+      // K order of a word: columns 0 2 4 6, then 1 3 5 7
+      if (e & 1) hi[p] |= ((uint32_t)d & 0xFFu) << (4 * (e & 6));
+      else lo[p] |= ((uint32_t)d & 0xFFu) << (4 * (e & 6));
+    }
+  }
+  uint8_t* half = op + (size_t)k * half_bytes;
+  uint8_t* dst = half + (word >> 2) * (n_cols * 32) + ((word >> 1) & 1) * 128 + (word & 1) * 8;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int c = 4 * n + p;
+    *reinterpret_cast<uint2*>(dst + (c >> 3) * 256 + (c & 7) * 16) = make_uint2(lo[p], hi[p]);
+  }
+  const int lanes = 16 / regions;
+  for (int o = 1; o < lanes; o <<= 1) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) sum[p] += __shfl_xor_sync(0xffffffffu, sum[p], o);
+  }
+  if (word % lanes == 0 && n < nbt) {
+    const int a01 = sum[0] * 256 + sum[1], a23 = sum[2] * 256 + sum[3];
+    const float unit = bad ? __int_as_float(0x7fffffff) : __uint_as_float((uint32_t)(E - 29 + 127) << 23);
+    *reinterpret_cast<int4*>(half + n_cols * kHalf + ((word / lanes) * nbt + n) * 16) =
+        make_int4(8 * a01, 8 * a23, __float_as_int(unit),
+                  __float_as_int((float)((double)a01 * 65536.0 + (double)a23)));
+  }
+}
+
+// The floating-point way. One block per half step; a thread takes 8 columns of a batch row and writes them,
 // permuted, as one 16-byte line of the operand (no-swizzle K-major: 8 rows x 16
 // bytes per core matrix, K step j of 16 columns at j * N * 32), for each part.
 // With minimums it also sums them per region (the 16 threads of a batch row
-// are neighbours). Rows nb .. N - 1 and columns past the matrix are zeros. The
-// first block clears the status and the tiles' counters.
+// are neighbours). Rows nb .. N - 1 and columns past the matrix are zeros.
 template <class X>
 __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx, int nb, int n_cols, int cols,
-                                                         int parts, int fold, int regions, uint8_t* op, float* xsum,
+                                                         int parts, int regions, uint8_t* op, float* xsum,
                                                          int* count, int tiles, int* status, int clear_status) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  clear_counts(count, tiles, status, clear_status);
   const int k = blockIdx.x, n = threadIdx.x >> 4, word = threadIdx.x & 15;
-  if (k == 0) {
-    if (threadIdx.x == 0 && clear_status) *status = NLS_OK;
-  }
-  for (int i = k * (int)blockDim.x + (int)threadIdx.x; i < tiles; i += (int)(gridDim.x * blockDim.x)) count[i] = 0;
   constexpr bool kF32 = std::is_same<X, float>::value;
   constexpr float kIn = std::is_same<X, __half>::value ? 1.0f : 0x1p-12f;
-  const int c0 = k * kHalf + word * 8;
   float v[8];
+  load8(x, ldx, nb, cols, n, k * kHalf + word * 8, v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  if (n < nb && c0 < cols) {  // (columns come in whole 32)
-    const X* p = x + (int64_t)n * ldx + c0;
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-      X t[8];
-#pragma unroll
-      for (int e = 0; e < (int)(8 * sizeof(X) / 16); ++e) reinterpret_cast<uint4*>(t)[e] = reinterpret_cast<const uint4*>(p)[e];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = to_f32(t[e]) * kIn;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = to_f32(p[e]) * kIn;
-    }
-  }
+  for (int e = 0; e < 8; ++e) v[e] *= kIn;
   if (xsum) {
     float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     const int lanes = 16 / regions;
@@ -170,15 +289,8 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
     if (word % lanes == 0) xsum[((size_t)k * regions + word / lanes) * n_cols + n] = s;
   }
   constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-  // fold > 0: part p of batch row n is column p * fold + n (columns past the
-  // parts are zeros: threads n >= fold write them)
-  uint8_t* dst = op + (size_t)k * (fold ? 1 : parts) * n_cols * (kHalf * 2) + (size_t)(word >> 1) * (n_cols * 32) +
-                 (word & 1) * 128;
-  auto line = [&](int c) { return dst + (c >> 3) * 256 + (c & 7) * 16; };
-  if (fold && n >= fold) {
-    if (n >= 3 * fold) *reinterpret_cast<uint4*>(line(n)) = make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
+  uint8_t* dst = op + (size_t)k * parts * n_cols * (kHalf * 2) + (size_t)(word >> 1) * (n_cols * 32) +
+                 (n >> 3) * 256 + (word & 1) * 128 + (n & 7) * 16;
 #pragma unroll
   for (int part = 0; part < (kF32 ? 3 : 1); ++part) {
     uint32_t w[4];
@@ -203,8 +315,7 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
       }
       w[j] = h[0] | (h[1] << 16);
     }
-    uint8_t* at = fold ? line(part * fold + n) : line(n) + (size_t)part * n_cols * (kHalf * 2);
-    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + (size_t)part * n_cols * (kHalf * 2)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -222,15 +333,25 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 // whole warp gets here with the same values: behind a branch of one lane the
 // operands would have to be moved to uniform registers one by one, which made
 // an issue cost about 110 cycles.
-template <bool ACC>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %4, 0;\n\t"
-      "setp.ne.u32 p, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(leader), "n"(ACC ? 1 : 0)
-      : "memory");
+template <bool I8, bool ACC>
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t leader) {
+  if constexpr (I8) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %4, 0;\n\t"
+        "setp.ne.u32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(leader), "n"(ACC ? 1 : 0)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %4, 0;\n\t"
+        "setp.ne.u32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(leader), "n"(ACC ? 1 : 0)
+        : "memory");
+  }
 }
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
@@ -272,16 +393,17 @@ __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t* r) {
   }
 }
 
-// the eight weights of a word as q - 8, in pairs (0, 4) (1, 5) (2, 6) (3, 7):
+// The eight weights of a word, low nibble first. Floating point: q - 8 in pairs
+// (0, 4) (1, 5) (2, 6) (3, 7):
 // a nibble under the exponent of 2^10 (fp16) or 2^7 (bfloat16) is that power
 // plus q, exactly; fp16's 10 bits of mantissa take the nibble at bit 4 too, as
-// 2^10 + 16 q
+// 2^10 + 16 q.
 template <bool BF16>
-struct Unpack {
+struct UnpackF {
   // the power of two's bits, out of the compiler's sight: as an immediate it
   // would take a logical operation of its own beside the mask's
   uint32_t magic;
-  __device__ __forceinline__ Unpack() { asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400)); }
+  __device__ __forceinline__ UnpackF() { asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400)); }
   template <uint32_t MASK>
   __device__ __forceinline__ uint32_t put(uint32_t w) const {
     uint32_t r;
@@ -311,6 +433,22 @@ struct Unpack {
       }
     }
   }
+};
+
+// Integers: q as bytes 0 2 4 6, then 1 3 5 7.
+struct UnpackI {
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t* o) const {
+    o[0] = w & 0x0F0F0F0Fu;
+    o[1] = (w >> 4) & 0x0F0F0F0Fu;
+  }
+};
+template <Op OP>
+struct UnpackOf {
+  using type = UnpackF<OP == Op::kBF16>;
+};
+template <>
+struct UnpackOf<Op::kI8> {
+  using type = UnpackI;
 };
 
 __device__ __forceinline__ float ld_scale(const uint8_t* base, int stype, int i) {
@@ -380,16 +518,18 @@ struct Ring {
   }
 };
 
-// NB: batch rows. R: groups per step. FOLD: the three parts of fp32 activations
-// are columns of their own (part p of batch row b in column NB p + b), else
-// further MMAs into the same columns.
-template <bool BF16, int NB, int R, bool FOLD>
+// NB: batch rows. R: groups per half step.
+template <Op OP, int NB, int R>
 __global__ void __launch_bounds__(kThreads, 1)
     g4_kernel(const KernelArgs a, const __grid_constant__ CUtensorMap qmap) {
-  constexpr int N = mma_n(NB);
-  constexpr int P = FOLD ? 3 : 1;
-  constexpr int kBuffers = 128 / (R * N) < kMaxBuffers ? 128 / (R * N) : kMaxBuffers;
-  static_assert(NB * P <= N && R * N <= 64 && kBuffers >= 2, "columns");
+  constexpr bool I8 = OP == Op::kI8;
+  constexpr int N = mma_n(OP, NB);
+  constexpr int kACols = a_cols(OP);                // of a tile half's operand
+  constexpr uint32_t kTmemD = 4 * kACols;           // the accumulators' first column
+  constexpr int kFit = acc_cols(OP) / (2 * R * N) & ~1;
+  constexpr int kBuffers = kFit < kMaxBuffers ? kFit : kMaxBuffers;
+  constexpr int kMmas = I8 ? 4 : 8;                 // per tile half and half step: K = 32 or 16
+  static_assert(NB * (I8 ? 4 : 1) <= N && kBuffers >= 2, "columns");
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars& B = *reinterpret_cast<Bars*>(smem + (size_t)a.stages * a.stage_bytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -442,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring slot{0, 1};
       const int per = R == 1 ? a.group / kHalf : 1;
       int g1 = 2 * k0 / per, left = per - 2 * k0 % per;
-      const uint32_t xb = (uint32_t)(a.parts * N * kStep * 2);
+      const uint32_t xb = (uint32_t)(2 * x_half(OP, NB, R, a.parts));
       for (int s = 0; s < nsteps; ++s) {
         if (s >= a.stages && !mbar_wait_bounded(&B.free[slot.i], slot.phase, a.wait_ns)) {
           fail = true;
@@ -483,10 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     fail = __any_sync(0xffffffffu, fail);
   } else if (warp == kMmaWarp) {
     const uint32_t leader = elect_one();
-    constexpr uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
+    // s32 += u8 x s8, or f32 += f16 x f16 (bf16 x bf16); both K-major
+    constexpr uint32_t kBF = OP == Op::kBF16 ? 1u : 0u;
+    constexpr uint32_t idesc = (I8 ? (2u << 4) | (1u << 10) : (1u << 4) | (kBF << 7) | (kBF << 10)) |
                                ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-    // no-swizzle K-major descriptor: 128 bytes from a row's first 8 columns to
-    // its next 8, 256 from 8 rows to the next
+    // no-swizzle K-major descriptor: 128 bytes from a row's first 16 bytes to
+    // its next 16, 256 from 8 rows to the next
     const uint64_t bd0 = (uint64_t)(((sbase + (uint32_t)a.x_off) >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) |
                          ((uint64_t)(256 >> 4) << 32) | ((uint64_t)1 << 46);
     Ring slot{0, 0}, buf{0, 1};  // stage; accumulators, with the phase of their last use
@@ -499,25 +641,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t bd = bd0 + (uint64_t)(slot.i * (a.stage_bytes >> 4) + h * a.parts * (N * kHalf * 2 / 16));
-        const uint32_t ab = tbase + (uint32_t)(h * 128), db = tbase + kTmemD + (uint32_t)(buf.i * (2 * R * N));
+        const uint64_t bd = bd0 + (uint64_t)(slot.i * (a.stage_bytes >> 4) + h * (x_half(OP, NB, R, a.parts) >> 4));
+        const uint32_t ab = tbase + (uint32_t)(h * 2 * kACols), db = tbase + kTmemD + (uint32_t)(buf.i * (2 * R * N));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j % (8 / R) == 0)
-              mma_f16<false>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
-            else
-              mma_f16<true>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bd + j * (N * 2), idesc, leader);
+          for (int j = 0; j < kMmas; ++j) {
+            const uint32_t d = db + (t * R + j * R / kMmas) * N, A = ab + t * kACols + 8 * j;
+            if (j % (kMmas / R) == 0) mma<I8, false>(d, A, bd + j * (N * 2), idesc, leader);
+            else mma<I8, true>(d, A, bd + j * (N * 2), idesc, leader);
           }
         }
-        for (int p = 1; p < a.parts; ++p) {
-          const uint64_t bp = bd + (uint64_t)(p * 8 * N * 2);
+        if constexpr (OP == Op::kBF16) {
+          for (int p = 1; p < a.parts; ++p) {
+            const uint64_t bp = bd + (uint64_t)(p * kMmas * N * 2);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              mma_f16<true>(db + (t * R + j * R / 8) * N, ab + t * 64 + 8 * j, bp + j * (N * 2), idesc, leader);
+              for (int j = 0; j < kMmas; ++j)
+                mma<I8, true>(db + (t * R + j * R / kMmas) * N, ab + t * kACols + 8 * j, bp + j * (N * 2), idesc, leader);
+          }
         }
         if (leader) {
           asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -533,14 +676,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < kUnpackWarps) {
     const int quarter = warp & 3, t = (warp >> 2) & 1, set = warp >> 3;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
-    const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(set * 128 + t * 64);
+    const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)((set * 2 + t) * kACols);
     const uint32_t bar = ready0 + (uint32_t)set * 8;
     // 16-byte pieces of a 128-byte row lie where the 128-byte swizzle of the
     // copy put them (free of bank conflicts)
     uint32_t at[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + (((4 * set + c) ^ (row & 7)) << 4));
-    const Unpack<BF16> unpack;
+    const typename UnpackOf<OP>::type unpack{};
+    constexpr int kWords = kACols / 16;     // operand words per packed word
+    constexpr int kPieces = 32 / (4 * kWords);  // 16-byte pieces per store of 32 words
     Ring slot{0, 0}, prev{set, 0};  // stage; accumulators of the step before's half
     for (int s = 0; s < nsteps; ++s) {
       if (!warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns)) {
@@ -550,17 +695,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t st = (uint32_t)(slot.i * a.stage_bytes);
       slot.next(a.stages);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kACols / 32; ++h) {
         uint32_t o[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kPieces; ++c) {
           uint32_t v[4];
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(at[2 * h + c] + st)
+                       : "r"(at[kPieces * h + c] + st)
                        : "memory");
 #pragma unroll
-          for (int i = 0; i < 4; ++i) unpack(v[i], o + 16 * c + 4 * i);
+          for (int i = 0; i < 4; ++i) unpack(v[i], o + (4 * c + i) * kWords);
         }
         // the step before had the same operand buffer
         if (h == 0 && s >= 1) {
@@ -602,39 +747,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d0 = td + (uint32_t)(buf.i * (2 * R * N));
         const int l0 = (2 * k + h) * R;  // the half's first line of scales
-        constexpr int C = NB < 8 ? NB : 8;
-        float sc[R];
+        float sc[R], mn[R];
+        auto scales = [&] {
 #pragma unroll
-        for (int c = 0; c < NB; c += C) {
-          uint32_t d[R][P][C];
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int p = 0; p < P; ++p) tmem_ld<C>(d0 + (uint32_t)(r * N + p * NB + c), d[r][p]);
-          if (c == 0) {
-#pragma unroll
-            for (int r = 0; r < R; ++r)  // (the last step may have fewer)
-              sc[r] = l0 + r < a.lines ? ld_scale(st + a.s_off, a.stype, (h * R + r) * kTile + row) : 0.0f;
+          for (int r = 0; r < R; ++r) {  // (the last step may have fewer)
+            const bool in = l0 + r < a.lines;
+            sc[r] = in ? ld_scale(st + a.s_off, a.stype, (h * R + r) * kTile + row) : 0.0f;
+            mn[r] = in && a.mins ? __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, (h * R + r) * kTile + row)) : 0.0f;
           }
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        };
+        if constexpr (I8) {
+          const int4* join = reinterpret_cast<const int4*>(st + a.x_off + h * x_half(OP, NB, R, 1) + N * kHalf);
+          constexpr int C = NB < 2 ? 1 : 2;  // batch rows per load
 #pragma unroll
-          for (int r = 0; r < R; ++r)
+          for (int c = 0; c < NB; c += C) {
+            uint32_t d[R][4 * C];
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-              float v = __uint_as_float(d[r][0][j]);
-              if constexpr (FOLD) v = (__uint_as_float(d[r][2][j]) + __uint_as_float(d[r][1][j])) + v;
-              acc[c + j] = __fmaf_rn(sc[r], v, acc[c + j]);
+            for (int r = 0; r < R; ++r) tmem_ld<4 * C>(d0 + (uint32_t)(r * N + 4 * c), d[r]);
+            if (c == 0) scales();
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int j = 0; j < C; ++j) {
+                // sum (q - 8) X: each pair of bytes' sums joined as integers
+                // (below 2^26 in magnitude), the pairs in fp32
+                const int4 e = join[r * NB + c + j];
+                const uint32_t* p = d[r] + 4 * j;
+                const int hi = (int)(p[0] * 256u + p[1]) - e.x, lo = (int)(p[2] * 256u + p[3]) - e.y;
+                float f = __fmul_rn(sc[r], __fmaf_rn(__int2float_rn(hi), 65536.0f, __int2float_rn(lo)));
+                if (a.mins) f = __fmaf_rn(mn[r], __int_as_float(e.w), f);
+                acc[c + j] = __fmaf_rn(f, __int_as_float(e.z), acc[c + j]);
+              }
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        } else {
+          constexpr int C = 8;
+#pragma unroll
+          for (int c = 0; c < NB; c += C) {
+            uint32_t d[R][C];
+#pragma unroll
+            for (int r = 0; r < R; ++r) tmem_ld<C>(d0 + (uint32_t)(r * N + c), d[r]);
+            if (c == 0) scales();
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int j = 0; j < C; ++j) acc[c + j] = __fmaf_rn(sc[r], __uint_as_float(d[r][j]), acc[c + j]);
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          if (a.mins) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              if (l0 + r >= a.lines) break;
+              const float* xs = a.xsum + (size_t)(l0 + r) * N;
+#pragma unroll
+              for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(mn[r], xs[j], acc[j]);
             }
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        if (a.mins) {
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            if (l0 + r >= a.lines) break;
-            const float m = __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, (h * R + r) * kTile + row));
-            const float* xs = a.xsum + (size_t)(l0 + r) * N;
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(m, xs[j], acc[j]);
           }
         }
         __syncwarp();
@@ -656,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int r = tile * kTile + row;
       bool write = true;
       if (first != 0 || k + 1 != a.ksteps) {
-        float* mine = a.part + (size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * N * kTile + row;
+        float* mine = a.part + (size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * NB * kTile + row;
 #pragma unroll
         for (int j = 0; j < NB; ++j) __stcg(mine + j * kTile, acc[j]);
         __threadfence();
@@ -687,16 +856,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           // every contributor's sums, in the order of the CTAs: the first is
           // the one whose steps hold the tile's first step
           const int64_t lo = (int64_t)tile * a.ksteps;
-          int c = (int)(((lo + 1) * gridDim.x - 1) / a.steps);
+          const int c0 = (int)(((lo + 1) * gridDim.x - 1) / a.steps);
+          const int c1 = (int)(((lo + a.ksteps) * gridDim.x - 1) / a.steps);
+          // (only the first's steps can begin before the tile; the loads of
+          // several are in flight together)
+          const float* theirs = a.part + (size_t)(2 * c0) * NB * kTile + row;
+          if (a.steps * c0 / gridDim.x < lo) theirs += NB * kTile;
 #pragma unroll
-          for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
-          for (;; ++c) {
-            const int64_t b0 = a.steps * c / gridDim.x;
-            if (b0 >= lo + a.ksteps) break;
-            const float* theirs = a.part + (size_t)(2 * c + (b0 >= lo ? 0 : 1)) * N * kTile + row;
+          for (int j = 0; j < NB; ++j) acc[j] = __ldcg(theirs + j * kTile);
+          constexpr int U = NB <= 2 ? 8 : NB <= 8 ? 4 : 1;
+          for (int c = c0 + 1; c <= c1; c += U) {
+            float v[U][NB];
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = __fadd_rn(acc[j], __ldcg(theirs + j * kTile));
-            if (c + 1 == (int)gridDim.x) break;
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int j = 0; j < NB; ++j)
+                v[u][j] = c + u <= c1 ? __ldcg(a.part + ((size_t)(2 * (c + u)) * NB + j) * kTile + row) : 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int j = 0; j < NB; ++j)
+                if (c + u <= c1) acc[j] = __fadd_rn(acc[j], v[u][j]);
           }
         }
       }
@@ -748,28 +928,42 @@ EncodeTiledFn encode_tiled() {
 }
 
 
-template <bool BF16, int R>
-const void* kernel_of(int nbt, bool fold) {
-  if constexpr (BF16) {
-    if (fold)
-      return nbt == 1 ? (const void*)g4_kernel<true, 1, R, true>
-             : nbt == 2 ? (const void*)g4_kernel<true, 2, R, true> : (const void*)g4_kernel<true, 4, R, true>;
-  }
-  switch (nbt) {
-    case 1: return (const void*)g4_kernel<BF16, 1, R, false>;
-    case 2: return (const void*)g4_kernel<BF16, 2, R, false>;
-    case 4: return (const void*)g4_kernel<BF16, 4, R, false>;
-    case 8: return (const void*)g4_kernel<BF16, 8, R, false>;
-    case 16: return (const void*)g4_kernel<BF16, 16, R, false>;
-  }
-  if constexpr (R <= 2) {
-    if (nbt == 32) return (const void*)g4_kernel<BF16, 32, R, false>;
-  }
-  if constexpr (R == 1) {
-    if (nbt == 48) return (const void*)g4_kernel<BF16, 48, R, false>;
-    if (nbt == 64) return (const void*)g4_kernel<BF16, 64, R, false>;
+template <Op OP, int R>
+const void* kernel_of(int nbt) {
+  if constexpr (OP == Op::kI8) {
+    switch (nbt) {
+      case 1: return (const void*)g4_kernel<OP, 1, R>;
+      case 2: return (const void*)g4_kernel<OP, 2, R>;
+      case 4: return (const void*)g4_kernel<OP, 4, R>;
+    }
+    if constexpr (i8_rows(R) >= 12) {
+      if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
+      if (nbt == 12) return (const void*)g4_kernel<OP, 12, R>;
+    }
+    if constexpr (i8_rows(R) >= 16) {
+      if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;
+    }
+  } else {
+    // (fewer rows than these are the integer way's)
+    if constexpr (i8_rows(R) < 8) {
+      if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
+    }
+    if constexpr (i8_rows(R) < 16) {
+      if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;
+    }
+    if constexpr (R <= 2) {
+      if (nbt == 32) return (const void*)g4_kernel<OP, 32, R>;
+    }
+    if constexpr (R == 1) {
+      if (nbt == 48) return (const void*)g4_kernel<OP, 48, R>;
+      if (nbt == 64) return (const void*)g4_kernel<OP, 64, R>;
+    }
   }
   return nullptr;
+}
+template <Op OP>
+const void* kernel_of(int regions, int nbt) {
+  return regions == 4 ? kernel_of<OP, 4>(nbt) : regions == 2 ? kernel_of<OP, 2>(nbt) : kernel_of<OP, 1>(nbt);
 }
 
 }  // namespace
@@ -802,42 +996,50 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   k.stype = a.stype;
   k.ssize = (int)dt_size(a.stype);
   k.x = ws;
-  k.xsum = a.mins ? reinterpret_cast<float*>(ws + p.x_bytes) : nullptr;
+  float* xsum = reinterpret_cast<float*>(ws + p.x_bytes);
   k.part = reinterpret_cast<float*>(ws + p.x_bytes + p.sum_bytes);
   k.count = reinterpret_cast<int*>(ws + p.x_bytes + p.sum_bytes + p.part_bytes);
   k.ytype = a.ytype;
   k.ldy = a.ldy;
-  k.out_scale = a.xtype == NLS_DT_F16 ? 1.0f : 4096.0f;
   k.ksteps = p.ksteps;
   k.steps = p.steps;
   k.wait_ns = a.wait_ns;
   k.status = a.status;
-  const bool bf16 = a.xtype != NLS_DT_F16;
   const size_t xes = dt_size(a.xtype), yes = dt_size(a.ytype);
-  for (int b0 = 0; b0 < a.nb; b0 += p.nmax) {
-    k.nb = std::min(p.nmax, a.nb - b0);
-    const int nbt = batch_of(k.nb), n = mma_n(nbt);
+  for (int b0 = 0; b0 < a.nb;) {
+    const Way w = way_of(a, a.nb - b0);
+    const bool i8 = w.op == Op::kI8;
+    const int half_bytes = x_half(w.op, w.nbt, p.regions, w.parts);
+    k.nb = w.nb;
+    k.parts = w.parts;
+    k.xsum = a.mins && !i8 ? xsum : nullptr;
+    k.out_scale = w.op == Op::kBF16 ? 4096.0f : 1.0f;
     k.y = static_cast<uint8_t*>(a.y) + (size_t)b0 * a.ldy * yes;
-    const bool fold = folded(p.parts, k.nb);
-    k.parts = fold ? 1 : p.parts;  // MMA passes over the columns
     k.x_off = kRawBytes;
-    k.s_off = k.x_off + k.parts * n * kStep * 2;
+    k.s_off = k.x_off + 2 * half_bytes;
     k.m_off = k.s_off + 2 * p.regions * kTile * k.ssize;
     k.stage_bytes = (k.m_off + (a.mins ? 2 * p.regions * kTile * k.ssize : 0) + 1023) & ~1023;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Bars);
     k.stages = std::min(kMaxStages, room / k.stage_bytes);
     const size_t smem = (size_t)k.stages * k.stage_bytes + sizeof(Bars);
-    const void* kern = p.regions == 4 ? (bf16 ? kernel_of<true, 4>(nbt, fold) : kernel_of<false, 4>(nbt, fold))
-                       : p.regions == 2 ? (bf16 ? kernel_of<true, 2>(nbt, fold) : kernel_of<false, 2>(nbt, fold))
-                                        : (bf16 ? kernel_of<true, 1>(nbt, fold) : kernel_of<false, 1>(nbt, fold));
+    const void* kern = i8 ? kernel_of<Op::kI8>(p.regions, w.nbt)
+                       : w.op == Op::kF16 ? kernel_of<Op::kF16>(p.regions, w.nbt)
+                                          : kernel_of<Op::kBF16>(p.regions, w.nbt);
     if (!kern) return cudaErrorInvalidValue;
     const void* x = static_cast<const uint8_t*>(a.x) + (size_t)b0 * a.ldx * xes;
+    const int clear = b0 == 0 ? 1 : 0;
     with_type(a.xtype, [&](auto xv) {
       using X = decltype(xv);
-      g4_layout_kernel<X><<<2 * p.ksteps, 16 * n, 0, st>>>(static_cast<const X*>(x), a.ldx, k.nb, n, a.cols, p.parts,
-                                                       fold ? nbt : 0, p.regions, ws, const_cast<float*>(k.xsum), k.count, p.tiles,
-                                                       a.status, b0 == 0);
+      if (i8)
+        g4_bytes_kernel<X><<<2 * p.ksteps, 4 * w.n, 0, st>>>(static_cast<const X*>(x), a.ldx, w.nb, w.nbt, w.n, a.cols,
+                                                             p.regions, ws, half_bytes, k.count, p.tiles, a.status,
+                                                             clear);
+      else
+        g4_layout_kernel<X><<<2 * p.ksteps, 16 * w.n, 0, st>>>(static_cast<const X*>(x), a.ldx, w.nb, w.n, a.cols,
+                                                               w.parts, p.regions, ws, const_cast<float*>(k.xsum),
+                                                               k.count, p.tiles, a.status, clear);
     });
+    b0 += w.nb;
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
