@@ -42,13 +42,13 @@
 // shape; a tile that more than one CTA worked on is joined by the last of them
 // to finish, from partial sums in the workspace added in CTA order (the same
 // bits every time; no CTA waits for another).
-// One CTA, 26 warps: 16 unpack in two sets, each one half of a step's columns (a
-// thread 128 columns of its row); 8 add the halves' sums to their rows'; one
-// issues the copies (a ring of stages: packed weights by tensor map,
-// activations, scales) and one the MMAs. Roles only wait for one another
-// through mbarriers, and each runs as far ahead as its buffers let it: operands
-// have one buffer per set in TMEM (2 x 128 columns), accumulators as many as
-// fit in the other 256 columns.
+// One CTA: 8 warps unpack (a thread its row's 256 columns, half after half), 8
+// or 16 add the halves' sums to their rows' (two sets, each one half of the
+// batch rows), one issues the copies (a ring of stages: packed weights by
+// tensor map, activations, scales) and one the MMAs. Roles only wait for one
+// another through mbarriers, and each runs as far ahead as its buffers let it:
+// operands have one buffer per half in TMEM, accumulators as many as fit in
+// the rest.
 #include <cuda.h>
 
 #include <algorithm>
@@ -66,17 +66,17 @@ namespace {
 constexpr int kTile = 256;       // weight rows per tile
 constexpr int kHalf = 128;       // columns per half of a step
 constexpr int kStep = 2 * kHalf;  // columns per step
-constexpr int kUnpackWarps = 16;  // two sets
-constexpr int kAddWarps = 8;
-constexpr int kCopyWarp = kUnpackWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kUnpackWarps = 8;
+// warps that add: one batch row leaves nothing for a second set
+__host__ __device__ constexpr int add_warps(int nbt) { return nbt == 1 ? 8 : 16; }
+__host__ __device__ constexpr int threads_of(int nbt) { return 32 * (kUnpackWarps + add_warps(nbt) + 2); }
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTmemCols = 512;
 
 enum class Op { kI8, kF16, kBF16 };
 // Tensor memory: a half step's operand takes 32 (bytes) or 64 columns per tile
-// half, two tile halves in each set's buffer; the rest are accumulators
+// half, two tile halves in each half step's buffer; the rest are accumulators
 __host__ __device__ constexpr int a_cols(Op op) { return op == Op::kI8 ? 32 : 64; }
 __host__ __device__ constexpr int acc_cols(Op op) { return (int)kTmemCols - 4 * a_cols(op); }
 
@@ -468,7 +468,7 @@ constexpr int kMaxBuffers = 8;  // accumulator buffers
 struct Bars {
   uint64_t full[kMaxStages];    // stage landed
   uint64_t free[kMaxStages];    // the step's sums are added (its MMAs are done, its scales read)
-  uint64_t ready[2];            // the set has stored its half's operand
+  uint64_t ready[2];            // a half's operand is stored
   uint64_t done[kMaxBuffers];   // a half's MMAs have completed
   uint64_t added[kMaxBuffers];  // its sums have been read
   uint64_t joined;              // every adding warp has written its partial sums
@@ -520,7 +520,7 @@ struct Ring {
 
 // NB: batch rows. R: groups per half step.
 template <Op OP, int NB, int R>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(NB), 1)
     g4_kernel(const KernelArgs a, const __grid_constant__ CUtensorMap qmap) {
   constexpr bool I8 = OP == Op::kI8;
   constexpr int N = mma_n(OP, NB);
@@ -529,6 +529,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kFit = acc_cols(OP) / (2 * R * N) & ~1;
   constexpr int kBuffers = kFit < kMaxBuffers ? kFit : kMaxBuffers;
   constexpr int kMmas = I8 ? 4 : 8;                 // per tile half and half step: K = 32 or 16
+  constexpr int kAddWarps = add_warps(NB);
+  constexpr int kCopyWarp = kUnpackWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
+  constexpr int CB = NB == 1 ? 1 : NB / 2;          // batch rows per adding thread
+  // A step's two halves are added together where that leaves the MMAs another
+  // step's accumulators (the waits and loads of a step are then one chain)
+  constexpr int kTogether = kBuffers >= 4 ? 2 : 1;
   static_assert(NB * (I8 ? 4 : 1) <= N && kBuffers >= 2, "columns");
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars& B = *reinterpret_cast<Bars*>(smem + (size_t)a.stages * a.stage_bytes);
@@ -545,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&B.full[i], 1);
       mbar_init(&B.free[i], kAddWarps);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&B.ready[i], kUnpackWarps / 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.ready[i], kUnpackWarps);
     for (int i = 0; i < kMaxBuffers; ++i) {
       mbar_init(&B.done[i], 1);
       mbar_init(&B.added[i], kAddWarps);
@@ -674,20 +680,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       slot.next(a.stages);
     }
   } else if (warp < kUnpackWarps) {
-    const int quarter = warp & 3, t = (warp >> 2) & 1, set = warp >> 3;
+    const int quarter = warp & 3, t = warp >> 2;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
-    const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)((set * 2 + t) * kACols);
-    const uint32_t bar = ready0 + (uint32_t)set * 8;
+    const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(t * kACols);
     // 16-byte pieces of a 128-byte row lie where the 128-byte swizzle of the
-    // copy put them (free of bank conflicts)
+    // copy put them (free of bank conflicts); the second half's 64 bytes on
     uint32_t at[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + (((4 * set + c) ^ (row & 7)) << 4));
+    for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
     const typename UnpackOf<OP>::type unpack{};
-    constexpr int kWords = kACols / 16;     // operand words per packed word
+    constexpr int kWords = kACols / 16;         // operand words per packed word
     constexpr int kPieces = 32 / (4 * kWords);  // 16-byte pieces per store of 32 words
-    Ring slot{0, 0}, prev{set, 0};  // stage; accumulators of the step before's half
-    for (int s = 0; s < nsteps; ++s) {
+    Ring slot{0, 0}, prev{0, 0};  // stage; accumulators of the half a step before
+    for (int s = 0; s < nsteps && !fail; ++s) {
       if (!warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns)) {
         fail = true;
         break;
@@ -695,123 +700,129 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t st = (uint32_t)(slot.i * a.stage_bytes);
       slot.next(a.stages);
 #pragma unroll
-      for (int h = 0; h < kACols / 32; ++h) {
-        uint32_t o[32];
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-          uint32_t v[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(at[kPieces * h + c] + st)
-                       : "memory");
+        for (int i = 0; i < kACols / 32; ++i) {
+          uint32_t o[32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) unpack(v[i], o + (4 * c + i) * kWords);
-        }
-        // the step before had the same operand buffer
-        if (h == 0 && s >= 1) {
-          if (!warp_wait(done0 + (uint32_t)prev.i * 8, prev.phase, a.wait_ns)) {
-            fail = true;
-            break;
+          for (int c = 0; c < kPieces; ++c) {
+            uint32_t v[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                         : "r"((at[kPieces * i + c] ^ (uint32_t)(h << 6)) + st)
+                         : "memory");
+#pragma unroll
+            for (int e = 0; e < 4; ++e) unpack(v[e], o + (4 * c + e) * kWords);
           }
-          prev.next(kBuffers, 2);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          // the step before had the same operand buffer
+          if (i == 0 && s >= 1) {
+            if (!warp_wait(done0 + (uint32_t)prev.i * 8, prev.phase, a.wait_ns)) {
+              fail = true;
+              break;
+            }
+            prev.next(kBuffers);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          tmem_st32(ta + h * 2 * kACols + i * 32, o);
         }
-        tmem_st32(ta + h * 32, o);
+        if (fail) break;
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(ready0 + (uint32_t)h * 8);
       }
-      if (fail) break;
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive(bar);
     }
   } else {
-    const int aw = warp - kUnpackWarps, quarter = aw & 3, t = aw >> 2;
+    const int aw = warp - kUnpackWarps, quarter = aw & 3, t = (aw >> 2) & 1, set = aw >> 3;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
-    const uint32_t td = tbase + ((uint32_t)(32 * quarter) << 16) + kTmemD + (uint32_t)(t * R * N);
-    float acc[NB];
+    const int b0 = set * CB;                        // its first batch row
+    const uint32_t td = tbase + ((uint32_t)(32 * quarter) << 16) + kTmemD + (uint32_t)(t * R * N + b0 * (I8 ? 4 : 1));
+    float acc[CB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < CB; ++j) acc[j] = 0.0f;
     int ends = 0;              // tiles joined so far (phase of the joining barriers)
     int tile = tile0, k = k0;  // position of the step
     Ring slot{0, 0}, buf{0, 0};
     for (int s = 0; s < nsteps; ++s) {
       const uint8_t* st = smem + (uint32_t)(slot.i * a.stage_bytes);
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        // (the stage has landed long since: that wait orders the scales' copies)
-        if (!warp_wait(done0 + (uint32_t)buf.i * 8, buf.phase, a.wait_ns) ||
-            (h == 0 && !warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns))) {
+      for (int h0 = 0; h0 < 2; h0 += kTogether) {
+        // the scales have landed with the stage
+        if (h0 == 0 && !warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns)) {
+          fail = true;
+          break;
+        }
+        float sc[kTogether][R], mn[kTogether][R];
+#pragma unroll
+        for (int h = 0; h < kTogether; ++h)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {  // (the last step may have fewer)
+            const int l = (h0 + h) * R + r;
+            const bool in = 2 * k * R + l < a.lines;
+            sc[h][r] = in ? ld_scale(st + a.s_off, a.stype, l * kTile + row) : 0.0f;
+            mn[h][r] = in && a.mins ? __fmaf_rn(8.0f, sc[h][r], ld_scale(st + a.m_off, a.stype, l * kTile + row)) : 0.0f;
+          }
+        // (the MMAs of the second half complete after the first's)
+        if (!warp_wait(done0 + (uint32_t)(buf.i + kTogether - 1) * 8, buf.phase, a.wait_ns)) {
           fail = true;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d0 = td + (uint32_t)(buf.i * (2 * R * N));
-        const int l0 = (2 * k + h) * R;  // the half's first line of scales
-        float sc[R], mn[R];
-        auto scales = [&] {
+        // batch rows per load: at most 32 words of sums at a time
+        constexpr int kWordsPer = (I8 ? 4 : 1) * R * kTogether;
+        constexpr int kMost = 32 / kWordsPer < (I8 ? 2 : 8) ? 32 / kWordsPer : (I8 ? 2 : 8);
+        constexpr int C = CB < kMost ? CB : kMost;
+        static_assert(CB % C == 0, "batch rows per load");
 #pragma unroll
-          for (int r = 0; r < R; ++r) {  // (the last step may have fewer)
-            const bool in = l0 + r < a.lines;
-            sc[r] = in ? ld_scale(st + a.s_off, a.stype, (h * R + r) * kTile + row) : 0.0f;
-            mn[r] = in && a.mins ? __fmaf_rn(8.0f, sc[r], ld_scale(st + a.m_off, a.stype, (h * R + r) * kTile + row)) : 0.0f;
-          }
-        };
-        if constexpr (I8) {
-          const int4* join = reinterpret_cast<const int4*>(st + a.x_off + h * x_half(OP, NB, R, 1) + N * kHalf);
-          constexpr int C = NB < 2 ? 1 : 2;  // batch rows per load
+        for (int c = 0; c < CB; c += C) {
+          uint32_t d[kTogether][R][C * (I8 ? 4 : 1)];
 #pragma unroll
-          for (int c = 0; c < NB; c += C) {
-            uint32_t d[R][4 * C];
+          for (int h = 0; h < kTogether; ++h)
 #pragma unroll
-            for (int r = 0; r < R; ++r) tmem_ld<4 * C>(d0 + (uint32_t)(r * N + 4 * c), d[r]);
-            if (c == 0) scales();
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            for (int r = 0; r < R; ++r)
+              tmem_ld<C * (I8 ? 4 : 1)>(td + (uint32_t)((buf.i + h) * (2 * R * N) + r * N + c * (I8 ? 4 : 1)), d[h][r]);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int h = 0; h < kTogether; ++h)
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
               for (int j = 0; j < C; ++j) {
-                // sum (q - 8) X: each pair of bytes' sums joined as integers
-                // (below 2^26 in magnitude), the pairs in fp32
-                const int4 e = join[r * NB + c + j];
-                const uint32_t* p = d[r] + 4 * j;
-                const int hi = (int)(p[0] * 256u + p[1]) - e.x, lo = (int)(p[2] * 256u + p[3]) - e.y;
-                float f = __fmul_rn(sc[r], __fmaf_rn(__int2float_rn(hi), 65536.0f, __int2float_rn(lo)));
-                if (a.mins) f = __fmaf_rn(mn[r], __int_as_float(e.w), f);
-                acc[c + j] = __fmaf_rn(f, __int_as_float(e.z), acc[c + j]);
+                if constexpr (I8) {
+                  // sum (q - 8) X: each pair of bytes' sums joined as integers
+                  // (below 2^26 in magnitude), the pairs in fp32
+                  const int4 e = *reinterpret_cast<const int4*>(st + a.x_off + (h0 + h) * x_half(OP, NB, R, 1) +
+                                                                N * kHalf + (r * NB + b0 + c + j) * 16);
+                  const uint32_t* p = d[h][r] + 4 * j;
+                  const int hi = (int)(p[0] * 256u + p[1]) - e.x, lo = (int)(p[2] * 256u + p[3]) - e.y;
+                  float f = __fmul_rn(sc[h][r], __fmaf_rn(__int2float_rn(hi), 65536.0f, __int2float_rn(lo)));
+                  if (a.mins) f = __fmaf_rn(mn[h][r], __int_as_float(e.w), f);
+                  acc[c + j] = __fmaf_rn(f, __int_as_float(e.z), acc[c + j]);
+                } else {
+                  acc[c + j] = __fmaf_rn(sc[h][r], __uint_as_float(d[h][r][j]), acc[c + j]);
+                }
               }
-          }
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        } else {
-          constexpr int C = 8;
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (!I8 && a.mins) {
 #pragma unroll
-          for (int c = 0; c < NB; c += C) {
-            uint32_t d[R][C];
-#pragma unroll
-            for (int r = 0; r < R; ++r) tmem_ld<C>(d0 + (uint32_t)(r * N + c), d[r]);
-            if (c == 0) scales();
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-              for (int j = 0; j < C; ++j) acc[c + j] = __fmaf_rn(sc[r], __uint_as_float(d[r][j]), acc[c + j]);
-          }
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          if (a.mins) {
+          for (int h = 0; h < kTogether; ++h)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-              if (l0 + r >= a.lines) break;
-              const float* xs = a.xsum + (size_t)(l0 + r) * N;
+              const int l = (2 * k + h0 + h) * R + r;
+              if (l >= a.lines) break;
+              const float* xs = a.xsum + (size_t)l * N + b0;
 #pragma unroll
-              for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(mn[r], xs[j], acc[j]);
+              for (int j = 0; j < CB; ++j) acc[j] = __fmaf_rn(mn[h][r], xs[j], acc[j]);
             }
-          }
         }
         __syncwarp();
         if (lane == 0) {
-          arrive(added0 + (uint32_t)buf.i * 8);
-          if (h == 1) arrive(free0 + (uint32_t)slot.i * 8);
+#pragma unroll
+          for (int h = 0; h < kTogether; ++h) arrive(added0 + (uint32_t)(buf.i + h) * 8);
+          if (h0 + kTogether == 2) arrive(free0 + (uint32_t)slot.i * 8);
         }
-        buf.next(kBuffers);
+        buf.next(kBuffers, kTogether);
       }
       if (fail) break;
       slot.next(a.stages);
@@ -825,9 +836,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int r = tile * kTile + row;
       bool write = true;
       if (first != 0 || k + 1 != a.ksteps) {
-        float* mine = a.part + (size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * NB * kTile + row;
+        float* mine = a.part + (size_t)(2 * blockIdx.x + (tile == tile0 ? 0 : 1)) * NB * kTile + (size_t)b0 * kTile + row;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) __stcg(mine + j * kTile, acc[j]);
+        for (int j = 0; j < CB; ++j) __stcg(mine + j * kTile, acc[j]);
         __threadfence();
         __syncwarp();
         if (lane == 0) arrive(smem_u32(&B.joined));
@@ -860,33 +871,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c1 = (int)(((lo + a.ksteps) * gridDim.x - 1) / a.steps);
           // (only the first's steps can begin before the tile; the loads of
           // several are in flight together)
-          const float* theirs = a.part + (size_t)(2 * c0) * NB * kTile + row;
+          const float* theirs = a.part + ((size_t)(2 * c0) * NB + b0) * kTile + row;
           if (a.steps * c0 / gridDim.x < lo) theirs += NB * kTile;
 #pragma unroll
-          for (int j = 0; j < NB; ++j) acc[j] = __ldcg(theirs + j * kTile);
-          constexpr int U = NB <= 2 ? 8 : NB <= 8 ? 4 : 1;
+          for (int j = 0; j < CB; ++j) acc[j] = __ldcg(theirs + j * kTile);
+          constexpr int U = CB <= 2 ? 8 : CB <= 8 ? 4 : 1;
           for (int c = c0 + 1; c <= c1; c += U) {
-            float v[U][NB];
+            float v[U][CB];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-              for (int j = 0; j < NB; ++j)
-                v[u][j] = c + u <= c1 ? __ldcg(a.part + ((size_t)(2 * (c + u)) * NB + j) * kTile + row) : 0.0f;
+              for (int j = 0; j < CB; ++j)
+                v[u][j] = c + u <= c1 ? __ldcg(a.part + ((size_t)(2 * (c + u)) * NB + b0 + j) * kTile + row) : 0.0f;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-              for (int j = 0; j < NB; ++j)
+              for (int j = 0; j < CB; ++j)
                 if (c + u <= c1) acc[j] = __fadd_rn(acc[j], v[u][j]);
           }
         }
       }
       if (write && r < a.rows) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-          if (j < a.nb) st_out(a.y, a.ytype, (int64_t)j * a.ldy + r, acc[j] * a.out_scale);
+        for (int j = 0; j < CB; ++j)
+          if (b0 + j < a.nb) st_out(a.y, a.ytype, (int64_t)(b0 + j) * a.ldy + r, acc[j] * a.out_scale);
       }
 #pragma unroll
-      for (int j = 0; j < NB; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < CB; ++j) acc[j] = 0.0f;
       ++tile;
       k = 0;
     }
@@ -1046,7 +1057,7 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3((unsigned)threads_of(w.nbt), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
