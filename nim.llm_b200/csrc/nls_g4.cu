@@ -42,9 +42,9 @@
 // shape; a tile that more than one CTA worked on is joined by the last of them
 // to finish, from partial sums in the workspace added in CTA order (the same
 // bits every time; no CTA waits for another).
-// One CTA: 8 warps unpack (a thread its row's 256 columns, half after half), 8
-// or 16 add the halves' sums to their rows' (two sets, each one half of the
-// batch rows), one issues the copies (a ring of stages: packed weights by
+// One CTA: 8 or 16 warps unpack (a thread its row's 256 columns, half after
+// half, or one half of them), 8 or 16 add the halves' sums to their rows' (16: two sets, each one half of
+// the batch rows), one issues the copies (a ring of stages: packed weights by
 // tensor map, activations, scales) and one the MMAs. Roles only wait for one
 // another through mbarriers, and each runs as far ahead as its buffers let it:
 // operands have one buffer per half in TMEM, accumulators as many as fit in
@@ -66,10 +66,7 @@ namespace {
 constexpr int kTile = 256;       // weight rows per tile
 constexpr int kHalf = 128;       // columns per half of a step
 constexpr int kStep = 2 * kHalf;  // columns per step
-constexpr int kUnpackWarps = 8;
-// warps that add: one batch row leaves nothing for a second set
-__host__ __device__ constexpr int add_warps(int nbt) { return nbt == 1 ? 8 : 16; }
-__host__ __device__ constexpr int threads_of(int nbt) { return 32 * (kUnpackWarps + add_warps(nbt) + 2); }
+
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTmemCols = 512;
@@ -80,19 +77,33 @@ enum class Op { kI8, kF16, kBF16 };
 __host__ __device__ constexpr int a_cols(Op op) { return op == Op::kI8 ? 32 : 64; }
 __host__ __device__ constexpr int acc_cols(Op op) { return (int)kTmemCols - 4 * a_cols(op); }
 
+// The split of a CTA's warps, 24 for unpacking and adding at most (72 registers
+// a thread). Unpacking bytes is cheap, and adding four sums per batch row is
+// not: 8 and 16 (one batch row leaves nothing for a second set). Unpacking to
+// 16 bits is the larger part up to 16 batch rows (88 us with 16 and 8, 100 with
+// 8 and 16, on 128256 x 4096); above, adding is (32 rows: 104 and 100 us).
+__host__ __device__ constexpr int unpack_warps(Op op, int nbt) { return op != Op::kI8 && nbt <= 16 ? 16 : 8; }
+__host__ __device__ constexpr int add_warps(Op op, int nbt) {
+  return op != Op::kI8 ? (nbt <= 16 ? 8 : 16) : nbt == 1 ? 8 : 16;
+}
+__host__ __device__ constexpr int threads_of(Op op, int nbt) { return 32 * (unpack_warps(op, nbt) + add_warps(op, nbt) + 2); }
+
 // groups (scales) per half step
 __host__ __device__ constexpr int regions_of(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
 // batch rows a launch is compiled for, and the MMA's columns
 __host__ __device__ constexpr int batch_of(Op op, int nb) {
-  if (op == Op::kI8) return nb <= 1 ? 1 : nb <= 2 ? 2 : nb <= 4 ? 4 : nb <= 8 ? 8 : nb <= 12 ? 12 : 16;
+  if (op == Op::kI8) return nb <= 1 ? 1 : nb <= 2 ? 2 : nb <= 4 ? 4 : nb <= 8 ? 8 : 12;
   return nb <= 8 ? 8 : nb <= 16 ? 16 : nb <= 32 ? 32 : nb <= 48 ? 48 : 64;
 }
 __host__ __device__ constexpr int mma_n(Op op, int nbt) {
   return op == Op::kI8 ? (nbt <= 4 ? 16 : 4 * nbt) : (nbt <= 16 ? 16 : nbt);
 }
-// The most batch rows the integer way takes: two buffers of accumulators have
-// to fit in tensor memory (96 columns per tile half and buffer).
-__host__ __device__ constexpr int i8_rows(int regions) { return regions == 4 ? 4 : regions == 2 ? 12 : 16; }
+// The most batch rows the integer way takes. Two buffers of accumulators have
+// to fit in tensor memory (96 columns per tile half and buffer): 4 rows with
+// groups of 32, 12 with groups of 64. With wider ones 12 too, by the times: 12 /
+// 16 rows take 82 / 112 us this way and 84 / 88 us in floating point (128256 x
+// 4096).
+__host__ __device__ constexpr int i8_rows(int regions) { return regions == 4 ? 4 : 12; }
 // bytes of a half step's laid-out activations: bytes (and per region and batch
 // row four words for the joining), or 16-bit parts
 __host__ __device__ constexpr int x_half(Op op, int nbt, int regions, int parts) {
@@ -520,7 +531,7 @@ struct Ring {
 
 // NB: batch rows. R: groups per half step.
 template <Op OP, int NB, int R>
-__global__ void __launch_bounds__(threads_of(NB), 1)
+__global__ void __launch_bounds__(threads_of(OP, NB), 1)
     g4_kernel(const KernelArgs a, const __grid_constant__ CUtensorMap qmap) {
   constexpr bool I8 = OP == Op::kI8;
   constexpr int N = mma_n(OP, NB);
@@ -529,9 +540,9 @@ __global__ void __launch_bounds__(threads_of(NB), 1)
   constexpr int kFit = acc_cols(OP) / (2 * R * N) & ~1;
   constexpr int kBuffers = kFit < kMaxBuffers ? kFit : kMaxBuffers;
   constexpr int kMmas = I8 ? 4 : 8;                 // per tile half and half step: K = 32 or 16
-  constexpr int kAddWarps = add_warps(NB);
+  constexpr int kUnpackWarps = unpack_warps(OP, NB), kAddWarps = add_warps(OP, NB);
   constexpr int kCopyWarp = kUnpackWarps + kAddWarps, kMmaWarp = kCopyWarp + 1;
-  constexpr int CB = NB == 1 ? 1 : NB / 2;          // batch rows per adding thread
+  constexpr int CB = NB * 8 / kAddWarps < 1 ? 1 : NB * 8 / kAddWarps;  // batch rows per adding thread
   // A step's two halves are added together where that leaves the MMAs another
   // step's accumulators (the waits and loads of a step are then one chain)
   constexpr int kTogether = kBuffers >= 4 ? 2 : 1;
@@ -551,7 +562,7 @@ __global__ void __launch_bounds__(threads_of(NB), 1)
       mbar_init(&B.full[i], 1);
       mbar_init(&B.free[i], kAddWarps);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&B.ready[i], kUnpackWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.ready[i], 8);
     for (int i = 0; i < kMaxBuffers; ++i) {
       mbar_init(&B.done[i], 1);
       mbar_init(&B.added[i], kAddWarps);
@@ -680,18 +691,20 @@ __global__ void __launch_bounds__(threads_of(NB), 1)
       slot.next(a.stages);
     }
   } else if (warp < kUnpackWarps) {
-    const int quarter = warp & 3, t = warp >> 2;
+    const int quarter = warp & 3, t = (warp >> 2) & 1;
     const int row = t * 128 + quarter * 32 + lane;  // in the tile
+    constexpr int kMine = 16 / kUnpackWarps;        // halves of a step it unpacks, from h1 on
+    const int h1 = kMine == 2 ? 0 : warp >> 3;
     const uint32_t ta = tbase + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(t * kACols);
     // 16-byte pieces of a 128-byte row lie where the 128-byte swizzle of the
     // copy put them (free of bank conflicts); the second half's 64 bytes on
     uint32_t at[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
+    for (int c = 0; c < 4; ++c) at[c] = sbase + (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4)) ^ (uint32_t)(h1 << 6);
     const typename UnpackOf<OP>::type unpack{};
     constexpr int kWords = kACols / 16;         // operand words per packed word
     constexpr int kPieces = 32 / (4 * kWords);  // 16-byte pieces per store of 32 words
-    Ring slot{0, 0}, prev{0, 0};  // stage; accumulators of the half a step before
+    Ring slot{0, 0}, prev{h1, 0};  // stage; accumulators of the half a step before
     for (int s = 0; s < nsteps && !fail; ++s) {
       if (!warp_wait(full0 + (uint32_t)slot.i * 8, slot.phase, a.wait_ns)) {
         fail = true;
@@ -700,7 +713,7 @@ __global__ void __launch_bounds__(threads_of(NB), 1)
       const uint32_t st = (uint32_t)(slot.i * a.stage_bytes);
       slot.next(a.stages);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kMine; ++h) {
 #pragma unroll
         for (int i = 0; i < kACols / 32; ++i) {
           uint32_t o[32];
@@ -720,16 +733,16 @@ __global__ void __launch_bounds__(threads_of(NB), 1)
               fail = true;
               break;
             }
-            prev.next(kBuffers);
+            prev.next(kBuffers, 2 / kMine);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
-          tmem_st32(ta + h * 2 * kACols + i * 32, o);
+          tmem_st32(ta + (uint32_t)((h1 + h) * 2 * kACols + i * 32), o);
         }
         if (fail) break;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) arrive(ready0 + (uint32_t)h * 8);
+        if (lane == 0) arrive(ready0 + (uint32_t)(h1 + h) * 8);
       }
     }
   } else {
@@ -951,17 +964,12 @@ const void* kernel_of(int nbt) {
       if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
       if (nbt == 12) return (const void*)g4_kernel<OP, 12, R>;
     }
-    if constexpr (i8_rows(R) >= 16) {
-      if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;
-    }
   } else {
     // (fewer rows than these are the integer way's)
     if constexpr (i8_rows(R) < 8) {
       if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
     }
-    if constexpr (i8_rows(R) < 16) {
-      if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;
-    }
+    if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;
     if constexpr (R <= 2) {
       if (nbt == 32) return (const void*)g4_kernel<OP, 32, R>;
     }
@@ -1057,7 +1065,7 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, 1, 1);
-    cfg.blockDim = dim3((unsigned)threads_of(w.nbt), 1, 1);
+    cfg.blockDim = dim3((unsigned)threads_of(w.op, w.nbt), 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
