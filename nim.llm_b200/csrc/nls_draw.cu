@@ -11,24 +11,31 @@
 // so their sums are exact whatever order they are added in, and a row has the
 // same token whatever its batch and cluster.
 //
-// One thread-block cluster per row; a CTA holds its slice of the row in shared
-// memory, so a logit is read from memory once. Then one of two ways:
-//  * Few candidates (top-k up to 512; min-p alone): a cut that at least the
-//    needed tokens reach -- for top-k a quantile of the threads' maxima, since
-//    the k-th largest of some of the logits is no larger than the k-th largest
-//    of all -- and the tokens above it, collected in the first CTA and sorted.
+// Where a row runs: with many rows, one CTA per row (four to an SM), which
+// streams the row from memory; with few, a thread-block cluster per row, each
+// CTA with its slice of the row in shared memory. Then one of two ways:
+//  * Few candidates (top-k up to 32 per warp; min-p alone): a cut that at least
+//    the needed tokens reach -- for top-k a quantile of the threads' maxima,
+//    since the k-th largest of some of the logits is no larger than the k-th
+//    largest of all -- and the tokens above it, collected and sorted by the
+//    (first) CTA. A streamed row takes the cut from its first logits and reads
+//    the row once.
 //  * Masses of the whole row (no top-k, or the candidates were too many):
 //    1024 bins over the row's span of logits get their tokens' masses (and
 //    counts, for top-k). The border of each prefix, and the token drawn, lie in
-//    known bins; their tokens are collected and sorted.
+//    known bins; their tokens are collected and sorted. A streamed row is read
+//    for its maximum, for the masses and for the tokens of those bins.
 // A bin that holds too many tokens (very many equal logits) sends the row to a
-// radix selection over comp, ten bits at a time, by the first CTA alone.
+// radix selection over comp, ten bits at a time, by the (first) CTA.
 // What bounds it: reading the logits for the first way; for the second the
 // fp64 operations of the masses (about 13 per logit at half rate) and two
 // shared-memory atomics per logit.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "nls_common.cuh"
 #include "nls_kernels.h"
@@ -40,15 +47,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;
 constexpr int kBins = 1024;
 constexpr int kIdxBits = 18;
 constexpr int kList = 2048;           // tokens the first CTA collects and sorts
 constexpr int kMine = 1024;           // tokens a CTA contributes at most
 constexpr double kUnit = 35184372088832.0;  // 2^45
-constexpr int kTopKMax = 512;         // top-k of the first way (16 warps x 32 maxima)
-constexpr size_t kSliceBytes = 68 * 1024;  // of a CTA's slice, so that two CTAs share an SM
+constexpr int kMaxWarps = 16;
 
 using u64 = unsigned long long;
 
@@ -71,11 +76,10 @@ struct Shared {
   u64 tot[kBins];
   uint32_t tcnt[kBins];
   double pow2[64];     // 2^(j / 64)
-  u64 red[kWarps];
+  u64 red[kMaxWarps];
   u64 sum[kMaxCluster], kept[kMaxCluster];  // the CTAs' masses: all, and at least min_p
   float top[kMaxCluster], low[kMaxCluster];
-  int bad[kMaxCluster];
-  float fred[2][kWarps];
+  float fred[2][kMaxWarps];
   Command cmd;
   unsigned n_list, n_mine;
   int pick;
@@ -111,6 +115,7 @@ struct Row {
   }
 };
 
+template <int NT>
 __device__ u64 block_sum(u64 v, Shared& S) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -119,11 +124,12 @@ __device__ u64 block_sum(u64 v, Shared& S) {
   __syncthreads();
   u64 t = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) t += S.red[w];
+  for (int w = 0; w < NT / 32; ++w) t += S.red[w];
   return t;
 }
 
 // the running sum of v over the threads before this one
+template <int NT>
 __device__ u64 block_scan(u64 v, Shared& S) {
   u64 x = v;
 #pragma unroll
@@ -136,32 +142,33 @@ __device__ u64 block_scan(u64 v, Shared& S) {
   __syncthreads();
   u64 t = x - v;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w)
+  for (int w = 0; w < NT / 32; ++w)
     if (w < (int)(threadIdx.x >> 5)) t += S.red[w];
   return t;
 }
 
 // the first bin whose running sum reaches target, or -1
-template <class V>
+template <int NT, class V>
 __device__ int first_bin(const V* run, double target, Shared& S) {
   __syncthreads();
   if (threadIdx.x == 0) S.pick = -1;
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kThreads)
+  for (int b = threadIdx.x; b < kBins; b += NT)
     if ((double)run[b] >= target && (b == 0 || (double)run[b - 1] < target)) S.pick = b;
   __syncthreads();
   return S.pick;
 }
 
 // S.list[0 .. n) ascending (n <= kList)
+template <int NT>
 __device__ void sort_list(int n, Shared& S) {
   int p = 32;
   while (p < n) p <<= 1;
-  for (int i = n + (int)threadIdx.x; i < p; i += kThreads) S.list[i] = ~0ull;
+  for (int i = n + (int)threadIdx.x; i < p; i += NT) S.list[i] = ~0ull;
   __syncthreads();
   for (int size = 2; size <= p; size <<= 1) {
     for (int stride = size >> 1; stride >= 32; stride >>= 1) {
-      for (int i = threadIdx.x; i < p / 2; i += kThreads) {
+      for (int i = threadIdx.x; i < p / 2; i += NT) {
         const int a = ((i & ~(stride - 1)) << 1) | (i & (stride - 1)), b = a + stride;
         const u64 x = S.list[a], y = S.list[b];
         if ((x > y) == ((a & size) == 0)) {
@@ -173,7 +180,7 @@ __device__ void sort_list(int n, Shared& S) {
     }
     // strides inside 32 neighbours: one warp, in registers
     const int lane = threadIdx.x & 31;
-    for (int base = 32 * (int)(threadIdx.x >> 5); base < p; base += kThreads) {
+    for (int base = 32 * (int)(threadIdx.x >> 5); base < p; base += NT) {
       u64 x = S.list[base + lane];
       for (int stride = min(size >> 1, 16); stride > 0; stride >>= 1) {
         const u64 y = __shfl_xor_sync(0xffffffffu, x, stride);
@@ -188,7 +195,7 @@ __device__ void sort_list(int n, Shared& S) {
 
 // Radix selection over the whole row in memory: the smallest comp whose running
 // count (by_count) or mass reaches target.
-template <class T>
+template <int NT, class T>
 __device__ u64 select(const T* x, int V, const Row& R, bool by_count, double target, Shared& S) {
   if (target < 1.0) target = 1.0;
   if (threadIdx.x == 0) {
@@ -196,10 +203,10 @@ __device__ u64 select(const T* x, int V, const Row& R, bool by_count, double tar
     S.before = 0;
   }
   for (int shift = 40; shift >= 0; shift -= 10) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) S.tot[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += NT) S.tot[i] = 0;
     __syncthreads();
     const u64 lo = S.lo, before = S.before;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
+    for (int i = threadIdx.x; i < V; i += NT) {
       const float v = to_f32(x[i]);
       const u64 d = Row::comp(v, i) - lo;
       if ((d >> (shift + 10)) == 0) {
@@ -208,18 +215,23 @@ __device__ u64 select(const T* x, int V, const Row& R, bool by_count, double tar
       }
     }
     __syncthreads();
-    const int b0 = 2 * threadIdx.x;
-    const u64 v0 = S.tot[b0], v1 = S.tot[b0 + 1];
-    const u64 e = before + block_scan(v0 + v1, S);
+    constexpr int kPer = kBins / NT;
+    const int b0 = kPer * threadIdx.x;
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += S.tot[b0 + i];
+    u64 e = before + block_scan<NT>(sum, S);
     __syncthreads();
     if (threadIdx.x == 0) S.pick = -1;
     __syncthreads();
-    if ((double)e < target && (double)(e + v0) >= target) {
-      S.pick = b0;
-      S.before = e;
-    } else if ((double)(e + v0) < target && (double)(e + v0 + v1) >= target) {
-      S.pick = b0 + 1;
-      S.before = e + v0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const u64 f = e + S.tot[b0 + i];
+      if ((double)e < target && (double)f >= target) {
+        S.pick = b0 + i;
+        S.before = e;
+      }
+      e = f;
     }
     __syncthreads();
     if (threadIdx.x == 0 && S.pick >= 0) S.lo = lo + ((u64)S.pick << shift);
@@ -231,27 +243,27 @@ __device__ u64 select(const T* x, int V, const Row& R, bool by_count, double tar
 }
 
 // The definition by radix selections, for rows that the ways above cannot take.
-template <class T>
+template <int NT, class T>
 __device__ u64 draw_slowly(const T* x, int V, const Row& R, const nls_draw_params& p, double u, double* kept, Shared& S) {
   u64 bound = ~0ull;  // what is kept: comp <= bound
-  if (p.top_k > 0 && p.top_k < V) bound = select(x, V, R, true, (double)p.top_k, S);
+  if (p.top_k > 0 && p.top_k < V) bound = select<NT>(x, V, R, true, (double)p.top_k, S);
   if (p.top_p > 0.0 && p.top_p < 1.0) {
     u64 t = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
+    for (int i = threadIdx.x; i < V; i += NT) {
       const float v = to_f32(x[i]);
       if (Row::comp(v, i) <= bound) t += Row::units(R.mass(v));
     }
-    const u64 c = select(x, V, R, false, p.top_p * (double)block_sum(t, S), S);
+    const u64 c = select<NT>(x, V, R, false, p.top_p * (double)block_sum<NT>(t, S), S);
     if (c < bound) bound = c;
   }
   u64 t = 0;
-  for (int i = threadIdx.x; i < V; i += kThreads) {
+  for (int i = threadIdx.x; i < V; i += NT) {
     const float v = to_f32(x[i]);
     const double m = R.mass(v);
     if (Row::comp(v, i) <= bound && !(p.min_p > 0.0 && m < p.min_p)) t += Row::units(m);
   }
-  *kept = (double)block_sum(t, S);
-  return select(x, V, R, false, u * *kept, S);
+  *kept = (double)block_sum<NT>(t, S);
+  return select<NT>(x, V, R, false, u * *kept, S);
 }
 
 // A vector of 16 bytes as fp32.
@@ -277,339 +289,423 @@ struct Vec {
   }
 };
 
+// the larger of two, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// the largest of a vector, NaN if it holds one
 template <class T>
-__global__ void __launch_bounds__(kThreads) draw_kernel(const DrawArgs a, int vchunk) {
-  constexpr int VN = Vec<T>::N;
+__device__ __forceinline__ float vec_max(const uint4& q) {
+  if constexpr (sizeof(T) == 4) {
+    return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)),
+                   max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* h = reinterpret_cast<const T2*>(&q);
+    const T2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(to_f32(m.x), to_f32(m.y));
+  }
+}
+
+// NT threads. STREAM: one CTA per row, the row read from memory on each pass;
+// else a cluster per row with vchunk 16-byte vectors of it per CTA.
+template <class T, int NT, bool STREAM>
+__global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, int vchunk) {
+  constexpr int VN = Vec<T>::N, kWarps = NT / 32;
+  constexpr int kPerBin = kBins / NT, kPerList = kList / NT;
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   uint4* slice = reinterpret_cast<uint4*>(smem + ((sizeof(Shared) + 15) & ~size_t(15)));
   const cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int C = STREAM ? 1 : (int)cluster.num_blocks(), rank = STREAM ? 0 : (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / (unsigned)C);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto remote = [&](int r) -> Shared& { return *cluster.map_shared_rank(&S, r); };
+  auto remote = [&](int r) -> Shared& { return STREAM ? S : *cluster.map_shared_rank(&S, r); };
+  auto sync_all = [&] {
+    if constexpr (STREAM) __syncthreads();
+    else cluster.sync();
+  };
 
-  if (tid == 0) {
-    S.n_list = 0;
-    S.n_mine = 0;
-  }
-  auto token = cluster.barrier_arrive();
+  if (tid == 0) S.n_list = S.n_mine = 0;
   if (tid < 64) S.pow2[tid] = exp2((double)tid / 64.0);
+  if constexpr (STREAM) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const nls_draw_params p = a.params[row];
+  const double u = a.uniforms ? a.uniforms[row] : -1.0;
+  const bool greedy = p.temperature <= 0.0 || p.min_p > 1.0;
+  const bool by_k = p.top_k > 0 && p.top_k < a.V, by_p = p.top_p > 0.0 && p.top_p < 1.0, by_m = p.min_p > 0.0;
+  // few candidates: top-k up to half the threads (the quantile of their maxima
+  // is near the k-th largest then), or min-p alone
+  const bool few = !greedy && ((by_k && p.top_k <= NT / 2) || (!by_k && !by_p && by_m));
 
-  // The slice: vectors [v0, v0 + nv) of the row, counted from the 16-byte
-  // boundary at or before its first logit. Vectors that reach past the row's
+  // The row, or the CTA's slice: vectors [v0, v0 + nv), counted from the 16-byte
+  // boundary at or before the first logit. Vectors that reach past the row's
   // ends are read by element; what is not the row's is -inf, which is never
   // drawn and has no mass.
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.ld;
   const int lead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int nvec = (lead + a.V + VN - 1) / VN;
-  const int v0 = rank * vchunk, nv = max(0, min(vchunk, nvec - v0));
+  const int v0 = STREAM ? 0 : rank * vchunk, nv = STREAM ? nvec : max(0, min(vchunk, nvec - v0));
   const uint4* xv = reinterpret_cast<const uint4*>(x - lead) + v0;
-  float top = -INFINITY, low = INFINITY;
-  int bad = 0;
-  auto take = [&](const uint4& q) {
-    const Vec<T> e(q);
+  auto load = [&](int i) -> uint4 {
+    const int first = (v0 + i) * VN - lead;  // the vector's first logit
+    if (i < nv && first >= 0 && first + VN <= a.V) return __ldg(xv + i);
+    union {
+      T e[VN];
+      uint4 v;
+    } w;
 #pragma unroll
-    for (int k = 0; k < VN; ++k) {
-      bad |= e.v[k] != e.v[k];
-      top = fmaxf(top, e.v[k]);
-      low = fminf(low, e.v[k] == -INFINITY ? INFINITY : e.v[k]);
+    for (int k = 0; k < VN; ++k)
+      w.e[k] = i < nv && first + k >= 0 && first + k < a.V ? x[first + k] : from_f32<T>(-INFINITY);
+    return w.v;
+  };
+  // f(i, vector i) for this thread's vectors, a whole warp together (i >= nv:
+  // -inf throughout)
+  constexpr int U = 4;  // loads in flight per thread and batch
+  auto vectors = [&](auto&& f) {
+    if constexpr (STREAM) {
+      for (int j = tid; j - lane < nv; j += U * NT) {
+        uint4 q[U];
+#pragma unroll
+        for (int t = 0; t < U; ++t) q[t] = load(j + t * NT);
+#pragma unroll
+        for (int t = 0; t < U; ++t) f(j + t * NT, q[t]);
+      }
+    } else {
+      for (int j = tid; j - lane < nv; j += NT) f(j, j < nv ? slice[j] : load(nv));
     }
   };
-  constexpr int U = 8;  // loads in flight per thread
-  for (int j = tid; j < nv; j += U * kThreads) {
-    uint4 q[U];
+
+  float top = -INFINITY, low = INFINITY, cut = -INFINITY;
+  int best = 0;  // the first vector that holds this thread's largest logit
+  // The cut that at least top_k of the logits seen reach: every warp's j-th
+  // largest of its threads' maxima, j = ceil(k / warps) (descending sort of 32;
+  // the warps are those whose threads all have logits), and the smallest of
+  // those. Or a little below max + T ln(min_p); the masses decide.
+  auto find_cut = [&] {
+    float m = top;
 #pragma unroll
-    for (int t = 0; t < U; ++t) {
-      const int i = j + t * kThreads;
-      const int first = (v0 + i) * VN - lead;  // the vector's first logit
-      if (i < nv && first >= 0 && first + VN <= a.V) {
-        q[t] = __ldcs(xv + i);
-      } else {
-        union {
-          T e[VN];
-          uint4 v;
-        } w;
+    for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-        for (int k = 0; k < VN; ++k)
-          w.e[k] = i < nv && first + k >= 0 && first + k < a.V ? x[first + k] : from_f32<T>(-INFINITY);
-        q[t] = w.v;
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        const float y = __shfl_xor_sync(0xffffffffu, m, stride);
+        m = ((lane & size) == 0) == ((lane & stride) == 0) ? fmaxf(m, y) : fminf(m, y);
       }
-    }
+    const int warps = min(kWarps, nv / 32), j = warps > 0 ? ((int)p.top_k + warps - 1) / warps : 33;
+    const float mj = __shfl_sync(0xffffffffu, m, by_k ? min(j, 32) - 1 : 0);
+    __syncthreads();
+    if (lane == 0) S.fred[0][warp] = mj;
+    __syncthreads();
+    float c = by_k ? INFINITY : -INFINITY;
 #pragma unroll
-    for (int t = 0; t < U; ++t) {
-      const int i = j + t * kThreads;
-      if (i < nv) slice[i] = q[t];
-      take(q[t]);
+    for (int w = 0; w < kWarps; ++w) {
+      if (!by_k) c = fmaxf(c, S.fred[0][w]);
+      else if (w < warps) c = fminf(c, S.fred[0][w]);
+    }
+    if (by_k) {
+      cut = j > 32 ? -INFINITY : c;
+    } else {
+      const float f = (float)((double)c + p.temperature * log(p.min_p));
+      cut = f == f ? f - fmaxf(fabsf(f), fabsf(c)) * 0x1p-20f : -INFINITY;
+    }
+  };
+  {
+    uint4 q[U], nx[U];
+#pragma unroll
+    for (int t = 0; t < U; ++t) q[t] = load(tid + t * NT);
+    for (int j0 = 0, batch = 0; j0 < nv; j0 += U * NT, ++batch) {
+      if (j0 + U * NT < nv) {
+#pragma unroll
+        for (int t = 0; t < U; ++t) nx[t] = load(tid + j0 + (U + t) * NT);
+      }
+      float vm[U];
+#pragma unroll
+      for (int t = 0; t < U; ++t) {
+        const int i = tid + j0 + t * NT;
+        if (!STREAM && i < nv) slice[i] = q[t];
+        vm[t] = vec_max<T>(q[t]);
+        if (STREAM && vm[t] > top) best = i;
+        top = max_nan(top, vm[t]);
+      }
+      if (batch == 0) {  // (the span of the bins need not be the whole row's)
+#pragma unroll
+        for (int t = 0; t < U; ++t) {
+          const Vec<T> e(q[t]);
+#pragma unroll
+          for (int k = 0; k < VN; ++k) low = fminf(low, e.v[k] == -INFINITY ? INFINITY : e.v[k]);
+        }
+      }
+      if (STREAM && few) {
+        // the cut rises as more of the row has been seen
+        if ((batch & (batch + 1)) == 0) find_cut();
+#pragma unroll
+        for (int t = 0; t < U; ++t) {
+          if (vm[t] >= cut && vm[t] > -INFINITY) {
+            const Vec<T> e(q[t]);
+            const int first = (tid + j0 + t * NT) * VN - lead;
+#pragma unroll
+            for (int k = 0; k < VN; ++k)
+              if (e.v[k] >= cut && e.v[k] > -INFINITY) {
+                const unsigned at = atomicAdd(&S.n_list, 1u);
+                if (at < kList) S.list[at] = Row::comp(e.v[k], first + k);
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < U; ++t) q[t] = nx[t];
     }
   }
+  if (!STREAM && few) find_cut();
   const float mine_top = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
+  __syncthreads();
   if (lane == 0) {
     S.fred[0][warp] = top;
     S.fred[1][warp] = low;
   }
-  bad = __syncthreads_or(bad);
+  __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    top = fmaxf(top, S.fred[0][w]);
+    top = max_nan(top, S.fred[0][w]);
     low = fminf(low, S.fred[1][w]);
   }
-  cluster.barrier_wait(std::move(token));  // every CTA has begun
-  if (tid < C) {
-    Shared& D = remote(tid);
-    D.top[rank] = top;
-    D.low[rank] = low;
-    D.bad[rank] = bad;
-  }
-  cluster.sync();
-  for (int r = 0; r < C; ++r) {
-    top = fmaxf(top, S.top[r]);
-    low = fminf(low, S.low[r]);
-    bad |= S.bad[r];
+  if constexpr (!STREAM) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has begun
+    if (tid < C) {
+      Shared& D = remote(tid);
+      D.top[rank] = top;
+      D.low[rank] = low;
+    }
+    cluster.sync();
+    for (int r = 0; r < C; ++r) {
+      top = max_nan(top, S.top[r]);
+      low = fminf(low, S.low[r]);
+    }
   }
 
-  const double u = a.uniforms ? a.uniforms[row] : -1.0;
-  const bool greedy = p.temperature <= 0.0;
   int err = NLS_OK;
-  if (bad || isinf(top)) err = NLS_ERR_NAN_LOGITS;
-  else if (!greedy && (!(p.temperature > 0.0) || !(u >= 0.0 && u < 1.0))) err = NLS_ERR_INVALID_ARG;
+  if (!(fabsf(top) < INFINITY)) err = NLS_ERR_NAN_LOGITS;
+  else if (!(p.temperature <= 0.0) && (!(p.temperature > 0.0) || !(u >= 0.0 && u < 1.0))) err = NLS_ERR_INVALID_ARG;
   auto finish = [&](int64_t id, float prob) {
-    if (tid == 0) {
-      a.out_ids[row] = id;
-      if (a.out_probs) a.out_probs[row] = prob;
-    }
+    a.out_ids[row] = id;
+    if (a.out_probs) a.out_probs[row] = prob;
   };
   if (err != NLS_OK) {  // (all CTAs agree; nothing remote is in flight)
-    if (rank == 0) {
+    if (rank == 0 && tid == 0) {
       finish(-1, 0.0f);
-      if (tid == 0) record_status(a.status, err);
+      record_status(a.status, err);
     }
     return;
   }
-  Row R;
-  R.mx = top;
-  R.inv_t = greedy ? 1.0 : fmin(1.0 / p.temperature, 1e300);
-  R.pow2 = S.pow2;
-  const bool by_k = p.top_k > 0 && p.top_k < a.V, by_p = p.top_p > 0.0 && p.top_p < 1.0, by_m = p.min_p > 0.0;
-
-  // f(logit, index) for the slice's logits above -inf
-  auto each = [&](auto&& f) {
-    for (int i = tid; i < nv; i += kThreads) {
-      const Vec<T> e(slice[i]);
-      const int first = (v0 + i) * VN - lead;
+  if (greedy) {
+    // the first of the highest logits
+    unsigned at = ~0u;
+    if constexpr (STREAM) {
+      if (mine_top == top) {
+        const Vec<T> e(load(best));
 #pragma unroll
-      for (int k = 0; k < VN; ++k) f(e.v[k], first + k);
-    }
-  };
-  // The tokens that pass `want`, into the first CTA's list (its count passes
-  // kList where they do not all fit). Ends with a cluster barrier.
-  auto collect = [&](auto&& want) {
-    __syncthreads();
-    for (int i0 = 32 * warp; i0 < nv; i0 += kThreads) {
-      const int i = i0 + lane;
-      const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-      const Vec<T> e(i < nv ? slice[i] : none);
-      const int first = (v0 + i) * VN - lead;
-      unsigned hits = 0;
-#pragma unroll
-      for (int k = 0; k < VN; ++k)
-        if (i < nv && e.v[k] > -INFINITY && want(e.v[k])) hits |= 1u << k;
-      if (__any_sync(0xffffffffu, hits)) {
-        int n = __popc(hits), at = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += y;
-        }
-        unsigned base = 0;
-        if (lane == 31) base = atomicAdd(&S.n_mine, (unsigned)at);
-        base = __shfl_sync(0xffffffffu, base, 31) + (unsigned)(at - n);
+        for (int k = VN - 1; k >= 0; --k)
+          if (e.v[k] == top) at = (unsigned)(best * VN - lead + k);
+      }
+    } else {
+      vectors([&](int i, const uint4& q) {
+        const Vec<T> e(q);
 #pragma unroll
         for (int k = 0; k < VN; ++k)
-          if (hits & (1u << k)) {
-            if (base < kMine) S.mine[base] = Row::comp(e.v[k], first + k);
-            ++base;
-          }
-      }
+          if (i < nv && e.v[k] == top) at = min(at, (unsigned)((v0 + i) * VN - lead + k));
+      });
     }
-    __syncthreads();
-    const unsigned n = S.n_mine;
-    Shared& D = remote(0);
-    if (tid == 0) S.value = atomicAdd(&D.n_list, n <= kMine ? n : (unsigned)kList + 1u);
-    __syncthreads();
-    if (tid == 0) S.n_mine = 0;
-    const unsigned at = (unsigned)S.value;
-    if (n <= kMine && at + n <= kList)
-      for (unsigned i = tid; i < n; i += kThreads) D.list[at + i] = S.mine[i];
-    cluster.sync();
-  };
-  // the first CTA's next command (the others' arguments are ignored)
-  auto command = [&](const Command& c) -> Command {
-    if (rank == 0 && tid < C) remote(tid).cmd = c;
-    cluster.sync();
-    return S.cmd;
-  };
-
-  if (greedy || p.min_p > 1.0) {
-    // the first of the highest logits
-    unsigned best = ~0u;
-    each([&](float v, int i) {
-      if (v == top) best = min(best, (unsigned)i);
-    });
-    best = __reduce_min_sync(0xffffffffu, best);
+    at = __reduce_min_sync(0xffffffffu, at);
     if (tid == 0) S.value = ~0ull;
     __syncthreads();
-    if (lane == 0 && best != ~0u) atomicMin(&S.value, (u64)best);
+    if (lane == 0) atomicMin(&S.value, (u64)at);
     __syncthreads();
     if (tid == 0) remote(0).sum[rank] = S.value;
-    cluster.sync();
-    if (rank == 0) {
+    sync_all();
+    if (rank == 0 && tid == 0) {
       u64 m = ~0ull;
       for (int r = 0; r < C; ++r) m = min(m, S.sum[r]);
       finish((int64_t)m, 1.0f);
     }
     return;
   }
+  Row R;
+  R.mx = top;
+  R.inv_t = fmin(1.0 / p.temperature, 1e300);
+  R.pow2 = S.pow2;
+
+  // The tokens that pass `want`, into the (first) CTA's list (its count passes
+  // kList where they do not all fit). Ends with a barrier of all.
+  auto collect = [&](auto&& want) {
+    __syncthreads();
+    vectors([&](int i, const uint4& q) {
+      const Vec<T> e(q);
+      const int first = (v0 + i) * VN - lead;
+#pragma unroll
+      for (int k = 0; k < VN; ++k)
+        if (e.v[k] > -INFINITY && i < nv && want(e.v[k])) {
+          const unsigned at = atomicAdd(STREAM ? &S.n_list : &S.n_mine, 1u);
+          if (STREAM) {
+            if (at < kList) S.list[at] = Row::comp(e.v[k], first + k);
+          } else {
+            if (at < kMine) S.mine[at] = Row::comp(e.v[k], first + k);
+          }
+        }
+    });
+    __syncthreads();
+    if constexpr (!STREAM) {
+      const unsigned n = S.n_mine;
+      Shared& D = remote(0);
+      if (tid == 0) S.value = atomicAdd(&D.n_list, n <= kMine ? n : (unsigned)kList + 1u);
+      __syncthreads();
+      if (tid == 0) S.n_mine = 0;
+      const unsigned at = (unsigned)S.value;
+      if (n <= kMine && at + n <= kList)
+        for (unsigned i = tid; i < n; i += NT) D.list[at + i] = S.mine[i];
+      cluster.sync();
+    }
+  };
+  // the first CTA's next command (the others' arguments are ignored)
+  auto command = [&](const Command& c) -> Command {
+    if constexpr (STREAM) return c;
+    if (rank == 0 && tid < C) remote(tid).cmd = c;
+    cluster.sync();
+    return S.cmd;
+  };
+
+  int n = 0;           // tokens in the list
+  u64 run[kPerList];   // the running masses of this thread's neighbours in it
+  // the first of them whose running mass reaches target: its place in the
+  // list (-1: none), and that mass in S.value
+  auto reach = [&](double target) -> int {
+    int at = INT_MAX;
+#pragma unroll
+    for (int k = kPerList - 1; k >= 0; --k)
+      if (kPerList * tid + k < n && (double)run[k] >= target) at = kPerList * tid + k;
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (tid == 0) S.pick = INT_MAX;
+    __syncthreads();
+    if (lane == 0 && at != INT_MAX) atomicMin(&S.pick, at);
+    __syncthreads();
+    const int i = S.pick;
+    if (i == INT_MAX) return -1;
+#pragma unroll
+    for (int k = 0; k < kPerList; ++k)
+      if (i == kPerList * tid + k) S.value = run[k];
+    __syncthreads();
+    return i;
+  };
+  auto give = [&](u64 c, double M) {
+    if (tid == 0)
+      finish((int64_t)(c & ((1u << kIdxBits) - 1)),
+             (float)(exp(((double)Row::value(c) - (double)top) * R.inv_t) * kUnit / M));
+  };
 
   // ---- few candidates ---------------------------------------------------------
-  if ((by_k && p.top_k <= kTopKMax) || (!by_k && !by_p && by_m)) {
-    float cut;
-    if (by_k) {
-      // every warp's j-th largest of its threads' maxima, j = ceil(k / warps): k
-      // logits of the slice reach the smallest of them (descending sort of 32;
-      // the warps are those whose threads all have logits)
-      const int warps = min(kWarps, nv / 32), j = warps > 0 ? ((int)p.top_k + warps - 1) / warps : 33;
-      float m = mine_top;
-#pragma unroll
-      for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-          const float y = __shfl_xor_sync(0xffffffffu, m, stride);
-          const bool down = (lane & size) == 0, lower = (lane & stride) == 0;
-          m = (down == lower) ? fmaxf(m, y) : fminf(m, y);
-        }
-      m = __shfl_sync(0xffffffffu, m, min(j, 32) - 1);
-      __syncthreads();
-      if (lane == 0) S.fred[0][warp] = m;
-      __syncthreads();
-      cut = INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) cut = w < warps ? fminf(cut, S.fred[0][w]) : cut;
-      if (j > 32) cut = -INFINITY;
-    } else {
-      // a little below max + T ln(min_p): the masses decide
-      const double d = (double)top + p.temperature * log(p.min_p);
-      const float f = (float)d;
-      cut = f == f ? f - fmaxf(fabsf(f), fabsf(top)) * 0x1p-20f : -INFINITY;
-    }
-    collect([&](float v) { return v >= cut; });
-    const unsigned n = S.n_list;
-    const Command c = command(Command{n <= kList ? kExit : kMasses, 0, 0, 0, 0});
+  if (few) {
+    if constexpr (!STREAM) collect([&](float v) { return v >= cut; });
+    const unsigned found = S.n_list;
+    const Command c = command(Command{found <= kList ? kExit : kMasses, 0, 0, 0, 0});
     if (c.op == kExit) {
       if (rank != 0) return;
-      sort_list((int)n, S);
-      int m = (int)n;  // tokens kept
-      if (by_k) m = min(m, (int)p.top_k);
-      // four neighbours per thread: their masses, running sums, and the steps
-      u64 w[4], run[4];
-      double ms[4];
+      sort_list<NT>((int)found, S);
+      n = by_k ? min((int)found, (int)p.top_k) : (int)found;  // tokens kept by top-k
       u64 t = 0;
+      unsigned enough = 0;  // which of them have at least min_p
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = 4 * tid + k;
-        ms[k] = i < m ? R.mass(Row::value(S.list[i])) : 0.0;
-        w[k] = Row::units(ms[k]);
-        t += w[k];
+      for (int k = 0; k < kPerList; ++k) {
+        const int i = kPerList * tid + k;
+        const double m = i < n ? R.mass(Row::value(S.list[i])) : 0.0;
+        if (!by_m || !(m < p.min_p)) enough |= 1u << k;
+        t += Row::units(m);
         run[k] = t;
       }
-      const u64 e = block_scan(t, S);
-      if (tid == 0) S.value = 0;
+      const u64 e = block_scan<NT>(t, S);
       __syncthreads();
-      if (tid == kThreads - 1) S.value = e + t;
+      if (tid == NT - 1) S.value = e + t;
       __syncthreads();
-      const double total = (double)S.value;
-      const double tp = by_p ? fmax(1.0, p.top_p * total) : 0.0;
-      // kept mass: the last token with what is before it short of top-p's
+      const double tp = by_p ? fmax(1.0, p.top_p * (double)S.value) : 0.0;
+      // the kept mass: the last token's with what is before it short of top-p's
       // mass, and at least min_p itself
-      u64 kept = 0;
+      u64 kept = 0, prev = e;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kPerList; ++k) {
         run[k] += e;
-        const bool in = 4 * tid + k < m && (!by_p || (double)(run[k] - w[k]) < tp) && (!by_m || !(ms[k] < p.min_p));
-        if (in) kept = run[k];
+        if (kPerList * tid + k < n && (!by_p || (double)prev < tp) && (enough & (1u << k))) kept = run[k];
+        prev = run[k];
       }
       __syncthreads();
       if (tid == 0) S.value = 0;
       __syncthreads();
       if (kept) atomicMax(&S.value, kept);
       __syncthreads();
-      const double M = (double)S.value, target = fmax(1.0, u * M);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if ((double)run[k] >= target && (double)(run[k] - w[k]) < target && 4 * tid + k < m) {
-          const u64 c1 = S.list[4 * tid + k];
-          a.out_ids[row] = (int64_t)(c1 & ((1u << kIdxBits) - 1));
-          if (a.out_probs)
-            a.out_probs[row] = (float)(exp(((double)Row::value(c1) - (double)top) * R.inv_t) * kUnit / M);
-        }
+      const double M = (double)S.value;
+      const int i = reach(fmax(1.0, u * M));
+      give(S.list[max(i, 0)], M);
       return;
     }
   }
 
   // ---- masses of the whole row ------------------------------------------------
   __syncthreads();
-  for (int i = tid; i < kBins; i += kThreads) S.h.lo[i] = S.h.hi[i] = S.h.cnt[i] = 0;
+  for (int i = tid; i < kBins; i += NT) S.h.lo[i] = S.h.hi[i] = S.h.cnt[i] = 0;
   if (tid == 0) S.n_list = 0;
   __syncthreads();
-  // logits below max - 32 T have no mass
+  // logits below max - 32 T have no mass; those below the span are in its last bin
   const float span = fminf(top - low, (float)(32.5 * p.temperature));
   const float scale = span > 0.0f ? (float)kBins / span : 0.0f;
   auto bin = [&](float v) { return min(kBins - 1, (int)((top - v) * scale)); };
   u64 all = 0, above = 0;
-  each([&](float v, int) {
-    const double m = R.mass(v);
-    const u64 w = Row::units(m);
-    all += w;
-    if (by_m && !(m < p.min_p)) above += w;
-    if (w) {
-      const int b = bin(v);
-      const uint32_t l = (uint32_t)w, was = atomicAdd(&S.h.lo[b], l);
-      const uint32_t h = (uint32_t)(w >> 32) + (was + l < was ? 1u : 0u);
-      if (h) atomicAdd(&S.h.hi[b], h);
-      if (by_k) atomicAdd(&S.h.cnt[b], 1u);
+  vectors([&](int, const uint4& q) {
+    const Vec<T> e(q);
+#pragma unroll
+    for (int k = 0; k < VN; ++k) {
+      const double m = R.mass(e.v[k]);
+      const u64 w = Row::units(m);
+      all += w;
+      if (by_m && !(m < p.min_p)) above += w;
+      if (w) {
+        const int b = bin(e.v[k]);
+        const uint32_t l = (uint32_t)w, was = atomicAdd(&S.h.lo[b], l);
+        const uint32_t h = (uint32_t)(w >> 32) + (was + l < was ? 1u : 0u);
+        if (h) atomicAdd(&S.h.hi[b], h);
+        if (by_k) atomicAdd(&S.h.cnt[b], 1u);
+      }
     }
   });
-  all = block_sum(all, S);
-  if (by_m) above = block_sum(above, S);
+  all = block_sum<NT>(all, S);
+  if (by_m) above = block_sum<NT>(above, S);
   if (tid == 0) {
     Shared& D = remote(0);
     D.sum[rank] = all;
     D.kept[rank] = above;
   }
-  cluster.sync();
+  sync_all();
   // each CTA adds up its share of the bins
   {
     Shared& D = remote(0);
     const int b0 = kBins * rank / C, b1 = kBins * (rank + 1) / C;
-    for (int b = b0 + tid; b < b1; b += kThreads) {
+    for (int b = b0 + tid; b < b1; b += NT) {
       u64 t = 0;
-      uint32_t n = 0;
+      uint32_t k = 0;
       for (int r = 0; r < C; ++r) {
         const Shared& F = remote(r);
         t += ((u64)F.h.hi[b] << 32) + F.h.lo[b];
-        if (by_k) n += F.h.cnt[b];
+        if (by_k) k += F.h.cnt[b];
       }
       D.tot[b] = t;
-      D.tcnt[b] = n;
+      D.tcnt[b] = k;
     }
   }
-  cluster.sync();
+  sync_all();
 
   if (rank != 0) {
     while (true) {
@@ -622,17 +718,19 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const DrawArgs a, int vc
     }
   }
 
-  // running sums of the bins (two per thread)
+  // running sums of the bins
   {
-    const u64 t0 = S.tot[2 * tid], t1 = S.tot[2 * tid + 1];
-    const u64 c0 = S.tcnt[2 * tid], c1 = S.tcnt[2 * tid + 1];
-    const u64 e = block_scan(t0 + t1, S);
-    S.tot[2 * tid] = e + t0;
-    S.tot[2 * tid + 1] = e + t0 + t1;
-    if (by_k) {
-      const u64 f = block_scan(c0 + c1, S);
-      S.tcnt[2 * tid] = (uint32_t)(f + c0);
-      S.tcnt[2 * tid + 1] = (uint32_t)(f + c0 + c1);
+    u64 t = 0, k = 0;
+#pragma unroll
+    for (int i = 0; i < kPerBin; ++i) {
+      t += S.tot[kPerBin * tid + i];
+      k += S.tcnt[kPerBin * tid + i];
+    }
+    u64 e = block_scan<NT>(t, S), f = by_k ? block_scan<NT>(k, S) : 0;
+#pragma unroll
+    for (int i = 0; i < kPerBin; ++i) {
+      S.tot[kPerBin * tid + i] = e += S.tot[kPerBin * tid + i];
+      S.tcnt[kPerBin * tid + i] = (uint32_t)(f += S.tcnt[kPerBin * tid + i]);
     }
     __syncthreads();
   }
@@ -643,10 +741,8 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const DrawArgs a, int vc
   }
   auto before = [&](int b) -> u64 { return b > 0 ? S.tot[b - 1] : 0ull; };
   // Collects the tokens of bins r0 .. r1 and q0 .. q1 (r1 < q0, or q1 < q0 for
-  // none) and sorts them; a thread's four neighbours then have their running
-  // mass in the row in run[] (and themselves in S.list). False: too many.
-  int n = 0;
-  u64 w[4], run[4];
+  // none) and sorts them; run[] are their running masses in the row. False:
+  // too many.
   auto gather = [&](int r0, int r1, int q0, int q1) -> bool {
     __syncthreads();
     if (tid == 0) S.n_list = 0;
@@ -657,65 +753,50 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const DrawArgs a, int vc
       return ((b >= r0 && b <= r1) || (b >= q0 && b <= q1)) && Row::units(R.mass(v)) != 0;
     });
     n = (int)S.n_list;
-    if (S.n_list > kList) return false;
-    sort_list(n, S);
+    if (n > kList) return false;
+    sort_list<NT>(n, S);
     u64 t = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = 4 * tid + k;
-      w[k] = i < n ? Row::units(R.mass(Row::value(S.list[i]))) : 0;
-      t += w[k];
+    for (int k = 0; k < kPerList; ++k) {
+      const int i = kPerList * tid + k;
+      if (i < n) t += Row::units(R.mass(Row::value(S.list[i])));
       run[k] = t;
     }
-    const u64 e = block_scan(t, S) + before(r0);
+    const u64 e = block_scan<NT>(t, S) + before(r0);
     const u64 gap = q0 <= q1 ? before(q0) - S.tot[r1] : 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = 4 * tid + k;
+    for (int k = 0; k < kPerList; ++k) {
+      const int i = kPerList * tid + k;
       run[k] += e;
       if (i < n && q0 <= q1 && bin(Row::value(S.list[i])) >= q0) run[k] += gap;
     }
     return true;
   };
-  // the collected token whose running mass is the first to reach target: its
-  // place in the list, and that mass in S.value
-  auto reach = [&](double target) -> int {
-    __syncthreads();
-    if (tid == 0) S.pick = -1;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (4 * tid + k < n && (double)run[k] >= target && (double)(run[k] - w[k]) < target) {
-        S.pick = 4 * tid + k;
-        S.value = run[k];
-      }
-    __syncthreads();
-    return S.pick;
-  };
 
   bool ok = true;
   if (by_k) {
-    const int b = first_bin(S.tcnt, (double)p.top_k, S);
+    const int b = first_bin<NT>(S.tcnt, (double)p.top_k, S);
     if (b >= 0) {  // (else all tokens with a mass are kept)
       ok = gather(b, b, 0, -1);
       if (ok) {
         const int i = (int)(p.top_k - 1) - (b > 0 ? (int)S.tcnt[b - 1] : 0);
         __syncthreads();
-        if (i / 4 == tid) S.value = run[i & 3];
+#pragma unroll
+        for (int k = 0; k < kPerList; ++k)
+          if (i == kPerList * tid + k) S.value = run[k];
         __syncthreads();
         total = S.value;
       }
     }
   }
-  u64 kept = by_m && at_least < total ? at_least : total;
   int i = -1;
-  double M = (double)kept;
+  double M = (double)(by_m && at_least < total ? at_least : total);
   if (ok && by_p) {
     const double tp = fmax(1.0, p.top_p * (double)total);
-    const int b = first_bin(S.tot, tp, S);
+    const int b = first_bin<NT>(S.tot, tp, S);
     // the kept mass lies in bin b: so does, mostly, the drawn token's bin
     const double m0 = fmin(M, fmax(tp, (double)before(b))), m1 = fmin(M, (double)S.tot[b]);
-    const int t0 = first_bin(S.tot, fmax(1.0, u * m0), S), t1 = first_bin(S.tot, fmax(1.0, u * m1), S);
+    const int t0 = first_bin<NT>(S.tot, fmax(1.0, u * m0), S), t1 = first_bin<NT>(S.tot, fmax(1.0, u * m1), S);
     ok = t1 + 1 >= b ? gather(t0, b, 0, -1) : gather(t0, t1, b, b);
     if (ok) {
       reach(tp);
@@ -731,26 +812,22 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const DrawArgs a, int vc
   }
   if (ok && i < 0) {
     const double target = fmax(1.0, u * M);
-    const int b = first_bin(S.tot, target, S);
+    const int b = first_bin<NT>(S.tot, target, S);
     ok = gather(b, b, 0, -1);
     if (ok) i = reach(target);
     ok = ok && i >= 0;
   }
   (void)command(Command{kExit, 0, 0, 0, 0});
-  u64 c1;
-  if (ok) {
-    c1 = S.list[i];
-  } else {
-    c1 = draw_slowly(x, a.V, R, p, u, &M, S);
-  }
-  const float prob = (float)(exp(((double)Row::value(c1) - (double)top) * R.inv_t) * kUnit / M);
-  finish((int64_t)(c1 & ((1u << kIdxBits) - 1)), prob);
+  give(ok ? S.list[i] : draw_slowly<NT>(x, a.V, R, p, u, &M, S), M);
 }
+
+constexpr int kStreamThreads = 256, kClusterThreads = 512;
+constexpr int kMaxSmem = 227 * 1024;
 
 size_t smem_bytes(int vchunk) { return ((sizeof(Shared) + 15) & ~size_t(15)) + (size_t)vchunk * 16; }
 
-std::atomic<int> g_smem_set[3][kMaxDevicesAttr];
-std::atomic<int> g_big_cluster[kMaxDevicesAttr];  // 0 unknown, 1 clusters of 8 at most, 2 of 16
+std::atomic<int> g_smem_set[2][3][kMaxDevicesAttr];
+std::atomic<int> g_big_cluster[3][kMaxDevicesAttr];  // 0 unknown, 1 clusters of 8 at most, 2 of 16
 
 }  // namespace
 
@@ -761,53 +838,60 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
   if (dev < 0 || dev >= kMaxDevicesAttr) return cudaErrorInvalidDevice;
   return with_type(a.ltype, [&](auto tv) -> cudaError_t {
     using T = decltype(tv);
-    const void* fn = reinterpret_cast<const void*>(draw_kernel<T>);
-    const int nvec = (a.V + 2 * (16 / (int)sizeof(T)) - 2) / (16 / (int)sizeof(T));  // with any lead
-    // As many CTAs per row as leave two of them room on an SM; more for a few
-    // rows, down to 128 vectors each
-    int C = (int)(((size_t)nvec * 16 + kSliceBytes - 1) / kSliceBytes);
-    const int spread = std::min(sm_count / std::max(1, a.rows), nvec / 128);
-    C = std::max(1, std::min(std::max(C, spread), kMaxCluster));
+    constexpr int VN = 16 / (int)sizeof(T);
+    const int nvec = (a.V + 2 * VN - 2) / VN;  // with any lead
+    const void* fn = reinterpret_cast<const void*>(draw_kernel<T, kClusterThreads, false>);
     cudaLaunchConfig_t cfg = {};
+    cfg.stream = st;
+    cudaError_t e = cudaSuccess;
+    // CTAs per row: what shares the SMs among the rows, at least 128 vectors
+    // each, at most 16 (8 where the device has no room for 16), and enough to
+    // hold the row. Rows that would not all be on the device at once so are
+    // streamed.
+    const int most = (kMaxSmem - (int)smem_bytes(0)) / 16;
+    const int need = (nvec + most - 1) / most;
+    int C = std::min({sm_count / std::max(1, a.rows), nvec / 128, kMaxCluster});
+    C = std::max({C, need, 1});
+    if ((int64_t)C * a.rows > sm_count && nvec > 128) {
+      const void* sfn = reinterpret_cast<const void*>(draw_kernel<T, kStreamThreads, true>);
+      e = ensure_smem_attr(sfn, (int)smem_bytes(0), g_smem_set[0][a.ltype]);
+      if (e != cudaSuccess) return e;
+      cfg.blockDim = dim3(kStreamThreads, 1, 1);
+      cfg.gridDim = dim3((unsigned)a.rows, 1, 1);
+      cfg.dynamicSmemBytes = smem_bytes(0);
+      return cudaLaunchKernelEx(&cfg, draw_kernel<T, kStreamThreads, true>, a, 0);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(kClusterThreads, 1, 1);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cfg.stream = st;
-    cudaError_t e = cudaSuccess;
     auto shape = [&] {
       attr[0].val.clusterDim.x = (unsigned)C;
       cfg.gridDim = dim3((unsigned)(a.rows * C), 1, 1);
       cfg.dynamicSmemBytes = smem_bytes((nvec + C - 1) / C);
-      e = ensure_smem_attr(fn, (int)cfg.dynamicSmemBytes, g_smem_set[sizeof(T) == 4 ? 0 : a.ltype]);
+      e = ensure_smem_attr(fn, (int)cfg.dynamicSmemBytes, g_smem_set[1][a.ltype]);
     };
     if (C > 8) {
-      int known = g_big_cluster[dev].load(std::memory_order_relaxed);
+      std::atomic<int>& big = g_big_cluster[a.ltype][dev];
+      int known = big.load(std::memory_order_relaxed);
       if (!known) {
         int n = 0;
         const int keep = C;
         C = kMaxCluster;
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(draw_kernel<float>),
-                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(draw_kernel<__half>),
-                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(reinterpret_cast<const void*>(draw_kernel<__nv_bfloat16>),
-                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) shape();
         known = e == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, fn, &cfg) == cudaSuccess && n >= 1 ? 2 : 1;
         (void)cudaGetLastError();
-        g_big_cluster[dev].store(known, std::memory_order_relaxed);
+        big.store(known, std::memory_order_relaxed);
         C = keep;
       }
-      if (known != 2) C = 8;
+      if (known != 2) C = std::max(8, need);
     }
     shape();
     if (e != cudaSuccess) return e;
-    return cudaLaunchKernelEx(&cfg, draw_kernel<T>, a, (nvec + C - 1) / C);
+    return cudaLaunchKernelEx(&cfg, draw_kernel<T, kClusterThreads, false>, a, (nvec + C - 1) / C);
   });
 }
 
