@@ -5,8 +5,8 @@
 // has the place of comp(i) = (complement of the logit's ordered key, i), a
 // 50-bit number. Every step of the definition keeps a prefix of that order, so
 // a row needs no sort: only the tokens near the borders of its prefixes do.
-// Masses are exp((x - max) / T) in fp64 (a table of 64 powers of two and a
-// polynomial of degree 5, after Tang, ACM TOMS 15(2), 1989; within 2^-47 of the
+// Masses are exp((x - max) / T) in fp64 (a table of 128 powers of two and a
+// polynomial of degree 4, after Tang, ACM TOMS 15(2), 1989; within 2^-48 of the
 // value), rounded to multiples of 2^-45: at most 2^18 of them sum below 2^63,
 // so their sums are exact whatever order they are added in, and a row has the
 // same token whatever its batch and cluster.
@@ -28,7 +28,7 @@
 // A bin that holds too many tokens (very many equal logits) sends the row to a
 // radix selection over comp, ten bits at a time, by the (first) CTA.
 // What bounds it: reading the logits for the first way; for the second the
-// fp64 operations of the masses (about 13 per logit at half rate) and two
+// fp64 operations of the masses (11 per logit at half rate) and two
 // shared-memory atomics per logit.
 #include <cooperative_groups.h>
 
@@ -53,7 +53,8 @@ constexpr int kIdxBits = 18;
 constexpr int kList = 2048;           // tokens the first CTA collects and sorts
 constexpr int kMine = 1024;           // tokens a CTA contributes at most
 constexpr double kUnit = 35184372088832.0;  // 2^45
-constexpr int kMaxWarps = 16;
+constexpr int kMaxWarps = 32;
+constexpr int kPow2 = 128;            // the exponential's table
 
 using u64 = unsigned long long;
 
@@ -75,9 +76,9 @@ struct Shared {
   // of the whole row, then their running sums (first CTA)
   u64 tot[kBins];
   uint32_t tcnt[kBins];
-  double pow2[64];     // 2^(j / 64)
+  double pow2[kPow2];  // 2^(j / 128)
   u64 red[kMaxWarps];
-  u64 sum[kMaxCluster], kept[kMaxCluster];  // the CTAs' masses: all, and at least min_p
+  u64 sum[kMaxCluster], kept[kMaxCluster];  // of each CTA: the first highest logit; mass of at least min_p
   float top[kMaxCluster], low[kMaxCluster];
   float fred[2][kMaxWarps];
   Command cmd;
@@ -88,31 +89,41 @@ struct Shared {
   u64 before;
 };
 
-// A row's logits and settings, and the arithmetic of its masses.
+// A row's largest logit and temperature, and the arithmetic of its masses.
 struct Row {
-  float mx;
-  double inv_t;
+  double top;          // the largest logit
+  double scale;        // 128 / (T ln 2)
+  float floor;         // logits below have no mass, -inf among them
   const double* pow2;
+  __device__ __forceinline__ Row(float mx, double T, const double* table) : top((double)mx), pow2(table) {
+    scale = __dmul_rn(fmin(1.0 / T, 1e300), 184.66496523378731);
+    // e^-36 is less than half a unit (the float nearest to max - 36 T is not
+    // above any that e^-32 lies above)
+    floor = fmaxf((float)__dsub_rn(top, __dmul_rn(36.0, T)), -3.402823466e38f);
+  }
   static __device__ __forceinline__ u64 comp(float v, int i) { return ((u64)(~fkey(v)) << kIdxBits) | (u64)i; }
   static __device__ __forceinline__ float value(u64 c) { return fkey_inv(~(uint32_t)(c >> kIdxBits)); }
-  // exp((v - max) / T), 0 below e^-32 (less than half a unit)
+  __device__ __forceinline__ bool has_mass(float v) const { return v >= floor; }
+  // exp((v - max) / T) = 2^(n / 128) 2^(f / 128), n whole, |f| <= 1/2, of a
+  // logit that has mass
   __device__ __forceinline__ double mass(float v) const {
-    const double z = __dmul_rn(__dsub_rn((double)v, (double)mx), inv_t);
-    if (!(z >= -32.0)) return 0.0;  // (-inf logits too)
-    const double kd = __fma_rn(z, 92.332482616893656768, 6755399441055744.0);  // z 64 / ln 2 + 1.5 2^52
-    const int k = __double2loint(kd);
-    const double r = __fma_rn(__dsub_rn(kd, 6755399441055744.0), -0.010830424696249145245, z);
-    const double r2 = __dmul_rn(r, r);
-    const double b = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0), c = __fma_rn(r, 1.0 / 6.0, 0.5);
-    const double p = __fma_rn(r2, __fma_rn(r2, b, c), r);  // e^r - 1
-    const double t = pow2[k & 63];
-    const double s = __hiloint2double(__double2hiint(t) + ((k >> 6) << 20), __double2loint(t));
-    return __fma_rn(s, p, s);
+    const double d = __dsub_rn((double)v, top);
+    const double kd = __fma_rn(d, scale, 6755399441055744.0);  // + 1.5 2^52: rounded to n
+    const int n = __double2loint(kd);
+    const double f = __fma_rn(d, scale, -__dsub_rn(kd, 6755399441055744.0));
+    constexpr double l = 0.0054152123481245725;  // ln 2 / 128
+    double p = __fma_rn(f, l * l * l * l / 24.0, l * l * l / 6.0);
+    p = __fma_rn(f, p, l * l / 2.0);
+    p = __fma_rn(f, p, l);
+    const double t = pow2[n & (kPow2 - 1)];
+    const double s = __hiloint2double(__double2hiint(t) + ((n >> 7) << 20), __double2loint(t));
+    return __fma_rn(s, __dmul_rn(f, p), s);
   }
   // in units of 2^-45: the low bits beside 1.5 2^7, whose last place they are
   static __device__ __forceinline__ u64 units(double m) {
     return (u64)(__double_as_longlong(__dadd_rn(m, 192.0)) - __double_as_longlong(192.0));
   }
+  __device__ __forceinline__ u64 units_of(float v) const { return has_mass(v) ? units(mass(v)) : 0ull; }
 };
 
 template <int NT>
@@ -210,7 +221,7 @@ __device__ u64 select(const T* x, int V, const Row& R, bool by_count, double tar
       const float v = to_f32(x[i]);
       const u64 d = Row::comp(v, i) - lo;
       if ((d >> (shift + 10)) == 0) {
-        const u64 w = by_count ? 1ull : Row::units(R.mass(v));
+        const u64 w = by_count ? 1ull : R.units_of(v);
         if (w) atomicAdd(&S.tot[d >> shift], w);
       }
     }
@@ -251,7 +262,7 @@ __device__ u64 draw_slowly(const T* x, int V, const Row& R, const nls_draw_param
     u64 t = 0;
     for (int i = threadIdx.x; i < V; i += NT) {
       const float v = to_f32(x[i]);
-      if (Row::comp(v, i) <= bound) t += Row::units(R.mass(v));
+      if (Row::comp(v, i) <= bound) t += R.units_of(v);
     }
     const u64 c = select<NT>(x, V, R, false, p.top_p * (double)block_sum<NT>(t, S), S);
     if (c < bound) bound = c;
@@ -259,8 +270,10 @@ __device__ u64 draw_slowly(const T* x, int V, const Row& R, const nls_draw_param
   u64 t = 0;
   for (int i = threadIdx.x; i < V; i += NT) {
     const float v = to_f32(x[i]);
-    const double m = R.mass(v);
-    if (Row::comp(v, i) <= bound && !(p.min_p > 0.0 && m < p.min_p)) t += Row::units(m);
+    if (R.has_mass(v) && Row::comp(v, i) <= bound) {
+      const double m = R.mass(v);
+      if (!(p.min_p > 0.0 && m < p.min_p)) t += Row::units(m);
+    }
   }
   *kept = (double)block_sum<NT>(t, S);
   return select<NT>(x, V, R, false, u * *kept, S);
@@ -312,9 +325,10 @@ __device__ __forceinline__ float vec_max(const uint4& q) {
 // NT threads. STREAM: one CTA per row, the row read from memory on each pass;
 // else a cluster per row with vchunk 16-byte vectors of it per CTA.
 template <class T, int NT, bool STREAM>
-__global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, int vchunk) {
+__global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const DrawArgs a, int vchunk) {
   constexpr int VN = Vec<T>::N, kWarps = NT / 32;
   constexpr int kPerBin = kBins / NT, kPerList = kList / NT;
+  static_assert(kPerBin >= 1 && kPow2 <= NT, "threads");
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   uint4* slice = reinterpret_cast<uint4*>(smem + ((sizeof(Shared) + 15) & ~size_t(15)));
@@ -329,7 +343,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   };
 
   if (tid == 0) S.n_list = S.n_mine = 0;
-  if (tid < 64) S.pow2[tid] = exp2((double)tid / 64.0);
+  if (tid < kPow2) S.pow2[tid] = exp2((double)tid / kPow2);
   if constexpr (STREAM) __syncthreads();
   else asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const nls_draw_params p = a.params[row];
@@ -363,15 +377,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   };
   // f(i, vector i) for this thread's vectors, a whole warp together (i >= nv:
   // -inf throughout)
-  constexpr int U = 4;  // loads in flight per thread and batch
+  constexpr int U = 16 / VN;  // loads per thread and batch (another batch is in flight)
   auto vectors = [&](auto&& f) {
     if constexpr (STREAM) {
+      uint4 q[U], nx[U];
+#pragma unroll
+      for (int t = 0; t < U; ++t) q[t] = load(tid + t * NT);
       for (int j = tid; j - lane < nv; j += U * NT) {
-        uint4 q[U];
+        if (j - lane + U * NT < nv) {
 #pragma unroll
-        for (int t = 0; t < U; ++t) q[t] = load(j + t * NT);
+          for (int t = 0; t < U; ++t) nx[t] = load(j + (U + t) * NT);
+        }
 #pragma unroll
-        for (int t = 0; t < U; ++t) f(j + t * NT, q[t]);
+        for (int t = 0; t < U; ++t) {
+          f(j + t * NT, q[t]);
+          q[t] = nx[t];
+        }
       }
     } else {
       for (int j = tid; j - lane < nv; j += NT) f(j, j < nv ? slice[j] : load(nv));
@@ -380,12 +401,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
 
   float top = -INFINITY, low = INFINITY, cut = -INFINITY;
   int best = 0;  // the first vector that holds this thread's largest logit
-  // The cut that at least top_k of the logits seen reach: every warp's j-th
-  // largest of its threads' maxima, j = ceil(k / warps) (descending sort of 32;
-  // the warps are those whose threads all have logits), and the smallest of
-  // those. Or a little below max + T ln(min_p); the masses decide.
-  auto find_cut = [&] {
-    float m = top;
+  // A cut that at least k of the block's values v (one per thread) reach, and
+  // not many more: every warp's j-th largest, j = ceil(k / warps) (descending
+  // sort of 32; the first `warps` warps have values throughout), the smallest of
+  // those, then bisection between it and the largest.
+  auto quantile = [&](float v, int k, int warps) -> float {
+    float m = v;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -393,25 +414,51 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
         const float y = __shfl_xor_sync(0xffffffffu, m, stride);
         m = ((lane & size) == 0) == ((lane & stride) == 0) ? fmaxf(m, y) : fminf(m, y);
       }
-    const int warps = min(kWarps, nv / 32), j = warps > 0 ? ((int)p.top_k + warps - 1) / warps : 33;
-    const float mj = __shfl_sync(0xffffffffu, m, by_k ? min(j, 32) - 1 : 0);
+    const int j = warps > 0 ? (k + warps - 1) / warps : 33;
+    const float mj = __shfl_sync(0xffffffffu, m, min(j, 32) - 1);
     __syncthreads();
-    if (lane == 0) S.fred[0][warp] = mj;
+    if (lane == 0) {
+      S.fred[0][warp] = mj;
+      S.fred[1][warp] = m;
+    }
     __syncthreads();
-    float c = by_k ? INFINITY : -INFINITY;
+    float c = INFINITY, d = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (!by_k) c = fmaxf(c, S.fred[0][w]);
-      else if (w < warps) c = fminf(c, S.fred[0][w]);
+      if (w < warps) c = fminf(c, S.fred[0][w]);
+      d = fmaxf(d, S.fred[1][w]);
     }
+    if (j > 32 || !(c > -INFINITY) || !(d < INFINITY)) return -INFINITY;
+    for (int i = 0; i < 10; ++i) {
+      const float mid = 0.5f * c + 0.5f * d;
+      if (!(mid > c && mid < d)) break;
+      const int reached = __syncthreads_count(v >= mid);
+      if (reached >= k) c = mid;
+      else d = mid;
+      if (reached >= k && reached <= k + k / 8) break;
+    }
+    return c;
+  };
+  // The cut of what this CTA has seen so far: of the threads' maxima for top-k;
+  // or a little below max + T ln(min_p) (the masses decide).
+  auto find_cut = [&] {
     if (by_k) {
-      cut = j > 32 ? -INFINITY : c;
+      cut = quantile(top, (int)p.top_k, min(kWarps, nv / 32));
     } else {
-      const float f = (float)((double)c + p.temperature * log(p.min_p));
-      cut = f == f ? f - fmaxf(fabsf(f), fabsf(c)) * 0x1p-20f : -INFINITY;
+      float m = top;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      __syncthreads();
+      if (lane == 0) S.fred[0][warp] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, S.fred[0][w]);
+      const float f = (float)((double)m + p.temperature * log(p.min_p));
+      cut = f == f ? f - fmaxf(fabsf(f), fabsf(m)) * 0x1p-20f : -INFINITY;
     }
   };
   {
+    constexpr int U = 4;
     uint4 q[U], nx[U];
 #pragma unroll
     for (int t = 0; t < U; ++t) q[t] = load(tid + t * NT);
@@ -536,10 +583,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
     }
     return;
   }
-  Row R;
-  R.mx = top;
-  R.inv_t = fmin(1.0 / p.temperature, 1e300);
-  R.pow2 = S.pow2;
+  const Row R(top, p.temperature, S.pow2);
 
   // The tokens that pass `want`, into the (first) CTA's list (its count passes
   // kList where they do not all fit). Ends with a barrier of all.
@@ -606,7 +650,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   auto give = [&](u64 c, double M) {
     if (tid == 0)
       finish((int64_t)(c & ((1u << kIdxBits) - 1)),
-             (float)(exp(((double)Row::value(c) - (double)top) * R.inv_t) * kUnit / M));
+             (float)(R.mass(Row::value(c)) * kUnit / M));
   };
 
   // ---- few candidates ---------------------------------------------------------
@@ -616,14 +660,37 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
     const Command c = command(Command{found <= kList ? kExit : kMasses, 0, 0, 0, 0});
     if (c.op == kExit) {
       if (rank != 0) return;
-      sort_list<NT>((int)found, S);
-      n = by_k ? min((int)found, (int)p.top_k) : (int)found;  // tokens kept by top-k
+      n = (int)found;
+      if (by_k && n > 2 * (int)p.top_k && n >= NT / 4) {
+        // most of the list is from cuts of less than the row: a cut of the list
+        float m = -INFINITY;
+        for (int i = tid; i < n; i += NT) m = fmaxf(m, Row::value(S.list[i]));
+        const float c = quantile(m, (int)p.top_k, min(kWarps, n / 32));
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+          const u64 v = S.list[i];
+          if (Row::value(v) >= c) {
+            const unsigned at = atomicAdd(&S.n_mine, 1u);
+            if (at < kMine) S.mine[at] = v;
+          }
+        }
+        __syncthreads();
+        const int left = (int)S.n_mine;
+        if (left <= kMine) {
+          n = left;
+          for (int i = tid; i < n; i += NT) S.list[i] = S.mine[i];
+        }
+        __syncthreads();
+      }
+      sort_list<NT>(n, S);
+      if (by_k) n = min(n, (int)p.top_k);  // tokens kept by top-k
       u64 t = 0;
       unsigned enough = 0;  // which of them have at least min_p
 #pragma unroll
       for (int k = 0; k < kPerList; ++k) {
         const int i = kPerList * tid + k;
-        const double m = i < n ? R.mass(Row::value(S.list[i])) : 0.0;
+        const float v = i < n ? Row::value(S.list[i]) : -INFINITY;
+        const double m = R.has_mass(v) ? R.mass(v) : 0.0;
         if (!by_m || !(m < p.min_p)) enough |= 1u << k;
         t += Row::units(m);
         run[k] = t;
@@ -659,35 +726,47 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   for (int i = tid; i < kBins; i += NT) S.h.lo[i] = S.h.hi[i] = S.h.cnt[i] = 0;
   if (tid == 0) S.n_list = 0;
   __syncthreads();
-  // logits below max - 32 T have no mass; those below the span are in its last bin
+  // A token's bin: its distance from the largest logit in 1023rds of the span,
+  // rounded to a whole number by adding 2^23 (logits below max - 32 T have no
+  // mass; those below the span are in the last bin).
   const float span = fminf(top - low, (float)(32.5 * p.temperature));
-  const float scale = span > 0.0f ? (float)kBins / span : 0.0f;
-  auto bin = [&](float v) { return min(kBins - 1, (int)((top - v) * scale)); };
-  u64 all = 0, above = 0;
-  vectors([&](int, const uint4& q) {
-    const Vec<T> e(q);
+  const float scale = span > 0.0f ? (float)(kBins - 1) / span : 0.0f;
+  constexpr int kZeroBin = 0x4B000000;  // 2^23
+  auto bin = [&](float v) {
+    return min(__float_as_int(__fmaf_rn(top - v, scale, 8388608.0f)), kZeroBin + kBins - 1) - kZeroBin;
+  };
+  u64 above = 0;  // the mass of tokens with at least min_p
+  auto masses = [&](auto with_m, auto with_k) {
+    vectors([&](int, const uint4& q) {
+      const Vec<T> e(q);
 #pragma unroll
-    for (int k = 0; k < VN; ++k) {
-      const double m = R.mass(e.v[k]);
-      const u64 w = Row::units(m);
-      all += w;
-      if (by_m && !(m < p.min_p)) above += w;
-      if (w) {
-        const int b = bin(e.v[k]);
-        const uint32_t l = (uint32_t)w, was = atomicAdd(&S.h.lo[b], l);
-        const uint32_t h = (uint32_t)(w >> 32) + (was + l < was ? 1u : 0u);
-        if (h) atomicAdd(&S.h.hi[b], h);
-        if (by_k) atomicAdd(&S.h.cnt[b], 1u);
+      for (int g = 0; g < VN; g += 4) {  // four at a time: independent chains
+        u64 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const double m = R.mass(e.v[g + k]);
+          w[k] = Row::units(m);
+          if (with_m.value && R.has_mass(e.v[g + k]) && !(m < p.min_p)) above += w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (R.has_mass(e.v[g + k])) {
+            const int b = bin(e.v[g + k]);
+            const uint32_t l = (uint32_t)w[k], was = atomicAdd(&S.h.lo[b], l);
+            const uint32_t h = (uint32_t)(w[k] >> 32) + (was + l < was ? 1u : 0u);
+            if (h) atomicAdd(&S.h.hi[b], h);
+            if (with_k.value) atomicAdd(&S.h.cnt[b], 1u);
+          }
       }
-    }
-  });
-  all = block_sum<NT>(all, S);
+    });
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (by_k) masses(Yes{}, Yes{});
+  else if (by_m) masses(Yes{}, No{});
+  else masses(No{}, No{});
   if (by_m) above = block_sum<NT>(above, S);
-  if (tid == 0) {
-    Shared& D = remote(0);
-    D.sum[rank] = all;
-    D.kept[rank] = above;
-  }
+  if (tid == 0) remote(0).kept[rank] = above;
   sync_all();
   // each CTA adds up its share of the bins
   {
@@ -707,14 +786,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   }
   sync_all();
 
+  // the tokens of bins r0 .. r1 and q0 .. q1 that have mass
+  auto collect_bins = [&](int r0, int r1, int q0, int q1) {
+    collect([&](float v) {
+      const int b = bin(v);
+      return ((b >= r0 && b <= r1) || (b >= q0 && b <= q1)) && R.has_mass(v);
+    });
+  };
   if (rank != 0) {
     while (true) {
       const Command c = command(Command{});
       if (c.op == kExit) return;
-      collect([&](float v) {
-        const int b = bin(v);
-        return ((b >= c.r0 && b <= c.r1) || (b >= c.q0 && b <= c.q1)) && Row::units(R.mass(v)) != 0;
-      });
+      collect_bins(c.r0, c.r1, c.q0, c.q1);
     }
   }
 
@@ -734,11 +817,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
     }
     __syncthreads();
   }
-  u64 total = 0, at_least = 0;
-  for (int r = 0; r < C; ++r) {
-    total += S.sum[r];
-    at_least += S.kept[r];
-  }
+  u64 total = S.tot[kBins - 1], at_least = 0;
+  for (int r = 0; r < C; ++r) at_least += S.kept[r];
   auto before = [&](int b) -> u64 { return b > 0 ? S.tot[b - 1] : 0ull; };
   // Collects the tokens of bins r0 .. r1 and q0 .. q1 (r1 < q0, or q1 < q0 for
   // none) and sorts them; run[] are their running masses in the row. False:
@@ -748,10 +828,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
     if (tid == 0) S.n_list = 0;
     __syncthreads();
     (void)command(Command{kGather, r0, r1, q0, q1});
-    collect([&](float v) {
-      const int b = bin(v);
-      return ((b >= r0 && b <= r1) || (b >= q0 && b <= q1)) && Row::units(R.mass(v)) != 0;
-    });
+    collect_bins(r0, r1, q0, q1);
     n = (int)S.n_list;
     if (n > kList) return false;
     sort_list<NT>(n, S);
@@ -759,7 +836,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
       const int i = kPerList * tid + k;
-      if (i < n) t += Row::units(R.mass(Row::value(S.list[i])));
+      if (i < n) t += R.units_of(Row::value(S.list[i]));
       run[k] = t;
     }
     const u64 e = block_scan<NT>(t, S) + before(r0);
@@ -821,13 +898,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) draw_kernel(const DrawArgs a, i
   give(ok ? S.list[i] : draw_slowly<NT>(x, a.V, R, p, u, &M, S), M);
 }
 
-constexpr int kStreamThreads = 256, kClusterThreads = 512;
 constexpr int kMaxSmem = 227 * 1024;
 
 size_t smem_bytes(int vchunk) { return ((sizeof(Shared) + 15) & ~size_t(15)) + (size_t)vchunk * 16; }
 
-std::atomic<int> g_smem_set[2][3][kMaxDevicesAttr];
-std::atomic<int> g_big_cluster[3][kMaxDevicesAttr];  // 0 unknown, 1 clusters of 8 at most, 2 of 16
+std::atomic<int> g_smem_set[4][3][kMaxDevicesAttr];
+std::atomic<int> g_big_cluster[2][3][kMaxDevicesAttr];  // 0 unknown, 1 clusters of 8 at most, 2 of 16
 
 }  // namespace
 
@@ -840,7 +916,6 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
     using T = decltype(tv);
     constexpr int VN = 16 / (int)sizeof(T);
     const int nvec = (a.V + 2 * VN - 2) / VN;  // with any lead
-    const void* fn = reinterpret_cast<const void*>(draw_kernel<T, kClusterThreads, false>);
     cudaLaunchConfig_t cfg = {};
     cfg.stream = st;
     cudaError_t e = cudaSuccess;
@@ -853,28 +928,38 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
     int C = std::min({sm_count / std::max(1, a.rows), nvec / 128, kMaxCluster});
     C = std::max({C, need, 1});
     if ((int64_t)C * a.rows > sm_count && nvec > 128) {
-      const void* sfn = reinterpret_cast<const void*>(draw_kernel<T, kStreamThreads, true>);
-      e = ensure_smem_attr(sfn, (int)smem_bytes(0), g_smem_set[0][a.ltype]);
-      if (e != cudaSuccess) return e;
-      cfg.blockDim = dim3(kStreamThreads, 1, 1);
-      cfg.gridDim = dim3((unsigned)a.rows, 1, 1);
-      cfg.dynamicSmemBytes = smem_bytes(0);
-      return cudaLaunchKernelEx(&cfg, draw_kernel<T, kStreamThreads, true>, a, 0);
+      // 1024 threads to an SM: four rows, or two where there are not that many
+      const bool many = a.rows > 3 * sm_count;
+      auto stream = [&](auto kernel, int threads, std::atomic<int>* set) {
+        cudaError_t f = ensure_smem_attr(reinterpret_cast<const void*>(kernel), (int)smem_bytes(0), set);
+        if (f != cudaSuccess) return f;
+        cfg.blockDim = dim3((unsigned)threads, 1, 1);
+        cfg.gridDim = dim3((unsigned)a.rows, 1, 1);
+        cfg.dynamicSmemBytes = smem_bytes(0);
+        return cudaLaunchKernelEx(&cfg, kernel, a, 0);
+      };
+      return many ? stream(draw_kernel<T, 256, true>, 256, g_smem_set[2][a.ltype])
+                  : stream(draw_kernel<T, 512, true>, 512, g_smem_set[3][a.ltype]);
     }
+    // one CTA per SM at most: 1024 threads, or 256 where a CTA's share is less
+    // than a vector for each of those
+    const int wide = (nvec + C - 1) / C > 1024 ? 1 : 0;
+    const auto kernel = wide ? draw_kernel<T, 1024, false> : draw_kernel<T, 256, false>;
+    const void* fn = reinterpret_cast<const void*>(kernel);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kClusterThreads, 1, 1);
+    cfg.blockDim = dim3(wide ? 1024u : 256u, 1, 1);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     auto shape = [&] {
       attr[0].val.clusterDim.x = (unsigned)C;
       cfg.gridDim = dim3((unsigned)(a.rows * C), 1, 1);
       cfg.dynamicSmemBytes = smem_bytes((nvec + C - 1) / C);
-      e = ensure_smem_attr(fn, (int)cfg.dynamicSmemBytes, g_smem_set[1][a.ltype]);
+      e = ensure_smem_attr(fn, (int)cfg.dynamicSmemBytes, g_smem_set[wide][a.ltype]);
     };
     if (C > 8) {
-      std::atomic<int>& big = g_big_cluster[a.ltype][dev];
+      std::atomic<int>& big = g_big_cluster[wide][a.ltype][dev];
       int known = big.load(std::memory_order_relaxed);
       if (!known) {
         int n = 0;
@@ -891,7 +976,7 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
     }
     shape();
     if (e != cudaSuccess) return e;
-    return cudaLaunchKernelEx(&cfg, draw_kernel<T, kClusterThreads, false>, a, (nvec + C - 1) / C);
+    return cudaLaunchKernelEx(&cfg, kernel, a, (nvec + C - 1) / C);
   });
 }
 
