@@ -5,11 +5,12 @@
 // has the place of comp(i) = (complement of the logit's ordered key, i), a
 // 50-bit number. Every step of the definition keeps a prefix of that order, so
 // a row needs no sort: only the tokens near the borders of its prefixes do.
-// Masses are exp((x - max) / T) in fp64 (a table of 128 powers of two and a
-// polynomial of degree 4, after Tang, ACM TOMS 15(2), 1989; within 2^-48 of the
-// value), rounded to multiples of 2^-45: at most 2^18 of them sum below 2^63,
-// so their sums are exact whatever order they are added in, and a row has the
-// same token whatever its batch and cluster.
+// Masses are exp((x - max) / T) in fp64 (a table of 512 powers of two and a
+// polynomial of degree 3, after Tang, ACM TOMS 15(2), 1989; within 2^-46 of the
+// value), rounded to multiples of 2^-45 as they are summed: at most 2^18 of them
+// stay below 2^63, and the sums are whole numbers, so their order does not
+// matter (but for a mass half way between two multiples, which may go to
+// either: 2^-45 of the largest).
 //
 // Where a row runs: with many rows, one CTA per row (four to an SM), which
 // streams the row from memory; with few, a thread-block cluster per row, each
@@ -20,16 +21,18 @@
 //    largest of all -- and the tokens above it, collected and sorted by the
 //    (first) CTA. A streamed row takes the cut from its first logits and reads
 //    the row once.
-//  * Masses of the whole row (no top-k, or the candidates were too many):
-//    1024 bins over the row's span of logits get their tokens' masses (and
-//    counts, for top-k). The border of each prefix, and the token drawn, lie in
-//    known bins; their tokens are collected and sorted. A streamed row is read
-//    for its maximum, for the masses and for the tokens of those bins.
-// A bin that holds too many tokens (very many equal logits) sends the row to a
-// radix selection over comp, ten bits at a time, by the (first) CTA.
+//  * Masses of the whole row (no top-k, or the candidates were too many): the
+//    masses of 1024 bins over the row's span of logits, to about 2^-13, say where
+//    the border of each prefix and the token drawn lie. One pass then sums the
+//    exact masses of the row and of what comes before those places, and collects
+//    the tokens there, which are sorted. (A token adds its mass relative to its
+//    bin's middle, by a polynomial of degree two in fp32, with one atomic.
+//    Binning the exact masses instead took 35 more instructions per logit and
+//    two returning atomics.) What the sums do not confirm, and bins that hold
+//    too many tokens (very many equal logits), goes to a radix selection over
+//    comp, ten bits at a time, by the (first) CTA.
 // What bounds it: reading the logits for the first way; for the second the
-// fp64 operations of the masses (11 per logit at half rate) and two
-// shared-memory atomics per logit.
+// instructions of the masses (about 11 of them fp64, at half rate, per logit).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -54,34 +57,45 @@ constexpr int kList = 2048;           // tokens the first CTA collects and sorts
 constexpr int kMine = 1024;           // tokens a CTA contributes at most
 constexpr double kUnit = 35184372088832.0;  // 2^45
 constexpr int kMaxWarps = 32;
-constexpr int kPow2 = 128;            // the exponential's table
+constexpr int kPow2 = 512;            // the exponential's table
 
 using u64 = unsigned long long;
 
 // What the first CTA tells the others.
 struct Command {
-  int op;              // kExit, kMasses or kGather
-  int r0, r1, q0, q1;  // kGather: the tokens of bins r0 .. r1 and q0 .. q1
+  int op;  // kExit, kMasses or kSums
+  // kSums: the masses of logits >= ra and >= qa (before the two ranges), the
+  // tokens from there down to rb and qb, the mass of logits >= enough
+  float ra, rb, qa, qb, enough;
 };
-constexpr int kExit = 0, kMasses = 1, kGather = 2;
+constexpr int kExit = 0, kMasses = 1, kSums = 2;
+struct Sums {
+  u64 all, enough;  // of the row; of its tokens with at least min_p
+  u64 before_r, before_q;
+};
 
 struct Shared {
   u64 list[kList];
   union {
-    struct {
-      uint32_t lo[kBins], hi[kBins], cnt[kBins];  // this CTA's bins
-    } h;
-    u64 mine[kMine];                              // its tokens for the list
+    // this CTA's bins: masses in 2^-13 of the middle's, and counts (for top-k)
+    uint32_t bins[2][kBins];
+    u64 mine[kMine];  // its tokens for the list
   };
-  // of the whole row, then their running sums (first CTA)
-  u64 tot[kBins];
-  uint32_t tcnt[kBins];
-  double pow2[kPow2];  // 2^(j / 128)
+  // (first CTA) running counts of the row's bins (of masses in 2^-13 before
+  // that), and running masses by estimate
+  uint32_t tcnt[kBins], tmass[kBins];
+  union {
+    double est[kBins];
+    u64 tot[kBins];       // radix selection
+  };
+  double pow2[kPow2];  // 2^(j / 512)
   u64 red[kMaxWarps];
-  u64 sum[kMaxCluster], kept[kMaxCluster];  // of each CTA: the first highest logit; mass of at least min_p
+  u64 first[kMaxCluster];  // each CTA's first highest logit
+  Sums sums[kMaxCluster];
   float top[kMaxCluster], low[kMaxCluster];
   float fred[2][kMaxWarps];
   Command cmd;
+  float ends[5];
   unsigned n_list, n_mine;
   int pick;
   u64 value;
@@ -92,11 +106,11 @@ struct Shared {
 // A row's largest logit and temperature, and the arithmetic of its masses.
 struct Row {
   double top;          // the largest logit
-  double scale;        // 128 / (T ln 2)
+  double scale;        // 512 / (T ln 2)
   float floor;         // logits below have no mass, -inf among them
   const double* pow2;
   __device__ __forceinline__ Row(float mx, double T, const double* table) : top((double)mx), pow2(table) {
-    scale = __dmul_rn(fmin(1.0 / T, 1e300), 184.66496523378731);
+    scale = __dmul_rn(fmin(1.0 / T, 1e300), 738.65986093514925);
     // e^-36 is less than half a unit (the float nearest to max - 36 T is not
     // above any that e^-32 lies above)
     floor = fmaxf((float)__dsub_rn(top, __dmul_rn(36.0, T)), -3.402823466e38f);
@@ -104,19 +118,17 @@ struct Row {
   static __device__ __forceinline__ u64 comp(float v, int i) { return ((u64)(~fkey(v)) << kIdxBits) | (u64)i; }
   static __device__ __forceinline__ float value(u64 c) { return fkey_inv(~(uint32_t)(c >> kIdxBits)); }
   __device__ __forceinline__ bool has_mass(float v) const { return v >= floor; }
-  // exp((v - max) / T) = 2^(n / 128) 2^(f / 128), n whole, |f| <= 1/2, of a
+  // exp((v - max) / T) = 2^(n / 512) e^(f ln 2 / 512), n whole, |f| <= 1/2, of a
   // logit that has mass
   __device__ __forceinline__ double mass(float v) const {
     const double d = __dsub_rn((double)v, top);
     const double kd = __fma_rn(d, scale, 6755399441055744.0);  // + 1.5 2^52: rounded to n
     const int n = __double2loint(kd);
     const double f = __fma_rn(d, scale, -__dsub_rn(kd, 6755399441055744.0));
-    constexpr double l = 0.0054152123481245725;  // ln 2 / 128
-    double p = __fma_rn(f, l * l * l * l / 24.0, l * l * l / 6.0);
-    p = __fma_rn(f, p, l * l / 2.0);
-    p = __fma_rn(f, p, l);
+    constexpr double l = 0.0013538030870311431;  // ln 2 / 512
+    const double p = __fma_rn(f, __fma_rn(f, l * l * l / 6.0, l * l / 2.0), l);
     const double t = pow2[n & (kPow2 - 1)];
-    const double s = __hiloint2double(__double2hiint(t) + ((n >> 7) << 20), __double2loint(t));
+    const double s = __hiloint2double(__double2hiint(t) + ((n >> 9) << 20), __double2loint(t));
     return __fma_rn(s, __dmul_rn(f, p), s);
   }
   // in units of 2^-45: the low bits beside 1.5 2^7, whose last place they are
@@ -328,7 +340,7 @@ template <class T, int NT, bool STREAM>
 __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const DrawArgs a, int vchunk) {
   constexpr int VN = Vec<T>::N, kWarps = NT / 32;
   constexpr int kPerBin = kBins / NT, kPerList = kList / NT;
-  static_assert(kPerBin >= 1 && kPow2 <= NT, "threads");
+  static_assert(kPerBin >= 1, "threads");
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& S = *reinterpret_cast<Shared*>(smem);
   uint4* slice = reinterpret_cast<uint4*>(smem + ((sizeof(Shared) + 15) & ~size_t(15)));
@@ -343,7 +355,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   };
 
   if (tid == 0) S.n_list = S.n_mine = 0;
-  if (tid < kPow2) S.pow2[tid] = exp2((double)tid / kPow2);
+  for (int i = tid; i < kPow2; i += NT) S.pow2[i] = exp2((double)i / kPow2);
   if constexpr (STREAM) __syncthreads();
   else asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const nls_draw_params p = a.params[row];
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       d = fmaxf(d, S.fred[1][w]);
     }
     if (j > 32 || !(c > -INFINITY) || !(d < INFINITY)) return -INFINITY;
-    for (int i = 0; i < 10; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const float mid = 0.5f * c + 0.5f * d;
       if (!(mid > c && mid < d)) break;
       const int reached = __syncthreads_count(v >= mid);
@@ -486,7 +498,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       }
       if (STREAM && few) {
         // the cut rises as more of the row has been seen
-        if ((batch & (batch + 1)) == 0) find_cut();
+        if (batch == 0 || batch == 3 || batch == 15 || batch == 63) find_cut();
 #pragma unroll
         for (int t = 0; t < U; ++t) {
           if (vm[t] >= cut && vm[t] > -INFINITY) {
@@ -574,35 +586,29 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     __syncthreads();
     if (lane == 0) atomicMin(&S.value, (u64)at);
     __syncthreads();
-    if (tid == 0) remote(0).sum[rank] = S.value;
+    if (tid == 0) remote(0).first[rank] = S.value;
     sync_all();
     if (rank == 0 && tid == 0) {
       u64 m = ~0ull;
-      for (int r = 0; r < C; ++r) m = min(m, S.sum[r]);
+      for (int r = 0; r < C; ++r) m = min(m, S.first[r]);
       finish((int64_t)m, 1.0f);
     }
     return;
   }
   const Row R(top, p.temperature, S.pow2);
 
-  // The tokens that pass `want`, into the (first) CTA's list (its count passes
-  // kList where they do not all fit). Ends with a barrier of all.
-  auto collect = [&](auto&& want) {
-    __syncthreads();
-    vectors([&](int i, const uint4& q) {
-      const Vec<T> e(q);
-      const int first = (v0 + i) * VN - lead;
-#pragma unroll
-      for (int k = 0; k < VN; ++k)
-        if (e.v[k] > -INFINITY && i < nv && want(e.v[k])) {
-          const unsigned at = atomicAdd(STREAM ? &S.n_list : &S.n_mine, 1u);
-          if (STREAM) {
-            if (at < kList) S.list[at] = Row::comp(e.v[k], first + k);
-          } else {
-            if (at < kMine) S.mine[at] = Row::comp(e.v[k], first + k);
-          }
-        }
-    });
+  // Tokens go to the (first) CTA's list (its count passes kList where they do
+  // not all fit): one by one by each thread, then, from the other CTAs' own
+  // lists, all together. The latter ends with a barrier of all.
+  auto put = [&](float v, int i) {
+    const unsigned at = atomicAdd(STREAM ? &S.n_list : &S.n_mine, 1u);
+    if (STREAM) {
+      if (at < kList) S.list[at] = Row::comp(v, i);
+    } else {
+      if (at < kMine) S.mine[at] = Row::comp(v, i);
+    }
+  };
+  auto hand_over = [&] {
     __syncthreads();
     if constexpr (!STREAM) {
       const unsigned n = S.n_mine;
@@ -655,9 +661,18 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 
   // ---- few candidates ---------------------------------------------------------
   if (few) {
-    if constexpr (!STREAM) collect([&](float v) { return v >= cut; });
+    if constexpr (!STREAM) {
+      vectors([&](int i, const uint4& q) {
+        if (!(vec_max<T>(q) >= cut)) return;
+        const Vec<T> e(q);
+#pragma unroll
+        for (int k = 0; k < VN; ++k)
+          if (e.v[k] >= cut && e.v[k] > -INFINITY) put(e.v[k], (v0 + i) * VN - lead + k);
+      });
+      hand_over();
+    }
     const unsigned found = S.n_list;
-    const Command c = command(Command{found <= kList ? kExit : kMasses, 0, 0, 0, 0});
+    const Command c = command(Command{found <= kList ? kExit : kMasses});
     if (c.op == kExit) {
       if (rank != 0) return;
       n = (int)found;
@@ -723,138 +738,244 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 
   // ---- masses of the whole row ------------------------------------------------
   __syncthreads();
-  for (int i = tid; i < kBins; i += NT) S.h.lo[i] = S.h.hi[i] = S.h.cnt[i] = 0;
-  if (tid == 0) S.n_list = 0;
+  for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;
   __syncthreads();
   // A token's bin: its distance from the largest logit in 1023rds of the span,
   // rounded to a whole number by adding 2^23 (logits below max - 32 T have no
-  // mass; those below the span are in the last bin).
-  const float span = fminf(top - low, (float)(32.5 * p.temperature));
-  const float scale = span > 0.0f ? (float)(kBins - 1) / span : 0.0f;
-  constexpr int kZeroBin = 0x4B000000;  // 2^23
-  auto bin = [&](float v) {
-    return min(__float_as_int(__fmaf_rn(top - v, scale, 8388608.0f)), kZeroBin + kBins - 1) - kZeroBin;
-  };
-  u64 above = 0;  // the mass of tokens with at least min_p
-  auto masses = [&](auto with_m, auto with_k) {
+  // mass; those below the span are in the last bin). The span is finite and not
+  // negative, whatever the temperature, and where the first logits seen are all
+  // -inf (low is +inf then).
+  const float widest = fminf((float)(32.5 * p.temperature), 3.402823466e38f);
+  const float span = low <= top ? fminf(top - low, widest) : widest;
+  const float scale = span > 1e-30f ? (float)(kBins - 1) / span : 0.0f;
+  constexpr float kWhole = 8388608.0f;  // 2^23
+  auto bin_of = [](float b) { return (int)min(__float_as_uint(b) - 0x4B000000u, (uint32_t)(kBins - 1)); };
+  auto bin = [&](float v) { return bin_of(__fmaf_rn(fminf(top - v, span), scale, kWhole)); };
+  // ln(mass) per bin
+  const double step = scale > 0.0f ? -1.0 / ((double)scale * p.temperature) : 0.0;
+  {
+    // 2^13 e^(step f) = 2^13 (1 + step f + (step f)^2 / 2), f the distance from
+    // the bin's middle in bins, as the low bits beside 2^23
+    const float c1 = (float)(8192.0 * step), c2 = (float)(4096.0 * step * step);
     vectors([&](int, const uint4& q) {
+      if (!R.has_mass(vec_max<T>(q))) return;
       const Vec<T> e(q);
 #pragma unroll
-      for (int g = 0; g < VN; g += 4) {  // four at a time: independent chains
-        u64 w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const double m = R.mass(e.v[g + k]);
-          w[k] = Row::units(m);
-          if (with_m.value && R.has_mass(e.v[g + k]) && !(m < p.min_p)) above += w[k];
+      for (int k = 0; k < VN; ++k)
+        if (R.has_mass(e.v[k])) {
+          const float d = fminf(top - e.v[k], span), b = __fmaf_rn(d, scale, kWhole);
+          const float f = __fmaf_rn(d, scale, kWhole - b);
+          const float w = __fmaf_rn(f, __fmaf_rn(f, c2, c1), kWhole + 8192.0f);
+          const int i = bin_of(b);
+          atomicAdd(&S.bins[0][i], __float_as_uint(w) - 0x4B000000u);
+          if (by_k) atomicAdd(&S.bins[1][i], 1u);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (R.has_mass(e.v[g + k])) {
-            const int b = bin(e.v[g + k]);
-            const uint32_t l = (uint32_t)w[k], was = atomicAdd(&S.h.lo[b], l);
-            const uint32_t h = (uint32_t)(w[k] >> 32) + (was + l < was ? 1u : 0u);
-            if (h) atomicAdd(&S.h.hi[b], h);
-            if (with_k.value) atomicAdd(&S.h.cnt[b], 1u);
-          }
-      }
     });
-  };
-  using Yes = std::true_type;
-  using No = std::false_type;
-  if (by_k) masses(Yes{}, Yes{});
-  else if (by_m) masses(Yes{}, No{});
-  else masses(No{}, No{});
-  if (by_m) above = block_sum<NT>(above, S);
-  if (tid == 0) remote(0).kept[rank] = above;
+  }
   sync_all();
   // each CTA adds up its share of the bins
   {
     Shared& D = remote(0);
     const int b0 = kBins * rank / C, b1 = kBins * (rank + 1) / C;
     for (int b = b0 + tid; b < b1; b += NT) {
-      u64 t = 0;
-      uint32_t k = 0;
+      uint32_t m = 0, k = 0;
       for (int r = 0; r < C; ++r) {
-        const Shared& F = remote(r);
-        t += ((u64)F.h.hi[b] << 32) + F.h.lo[b];
-        if (by_k) k += F.h.cnt[b];
+        m += remote(r).bins[0][b];
+        if (by_k) k += remote(r).bins[1][b];
       }
-      D.tot[b] = t;
-      D.tcnt[b] = k;
+      D.tmass[b] = m;
+      D.tcnt[b] = by_k ? k : (m + 4096u) >> 13;  // (nearly, where no count has to be exact)
     }
   }
   sync_all();
 
-  // the tokens of bins r0 .. r1 and q0 .. q1 that have mass
-  auto collect_bins = [&](int r0, int r1, int q0, int q1) {
-    collect([&](float v) {
-      const int b = bin(v);
-      return ((b >= r0 && b <= r1) || (b >= q0 && b <= q1)) && R.has_mass(v);
-    });
+  // The sums and tokens of a command, into the first CTA. Ends with a barrier
+  // of all.
+  auto add_up = [&](const Command& c) {
+    Sums z{0, 0, 0, 0};
+    const bool two = c.qb < c.qa;  // a second range
+    __syncthreads();
+    auto pass = [&](auto with_m, auto with_q) {
+      vectors([&](int i, const uint4& q) {
+        if (!__any_sync(0xffffffffu, R.has_mass(vec_max<T>(q)))) return;
+        const Vec<T> e(q);
+        // (192 = 1.5 2^7: its last place is a unit, and a vector's masses do not
+        // change its exponent)
+        double all = 192.0, before_r = 192.0, before_q = 192.0, enough = 192.0;
+        unsigned hits = 0;
+#pragma unroll
+        for (int k = 0; k < VN; ++k) {
+          const float v = e.v[k];
+          const double m = R.mass(v);
+          if (R.has_mass(v)) all = __dadd_rn(all, m);
+          if (v >= c.ra) before_r = __dadd_rn(before_r, m);
+          if (with_m.value && v >= c.enough) enough = __dadd_rn(enough, m);
+          if (v >= c.rb && !(v >= c.ra)) hits |= 1u << k;
+          if (with_q.value) {
+            if (v >= c.qa) before_q = __dadd_rn(before_q, m);
+            if (v >= c.qb && !(v >= c.qa)) hits |= 1u << k;
+          }
+        }
+        auto units = [](double x) { return (u64)(__double_as_longlong(x) - __double_as_longlong(192.0)); };
+        z.all += units(all);
+        z.before_r += units(before_r);
+        if (with_m.value) z.enough += units(enough);
+        if (with_q.value) z.before_q += units(before_q);
+        if (hits) {
+#pragma unroll
+          for (int k = 0; k < VN; ++k)
+            if (hits & (1u << k)) put(e.v[k], (v0 + i) * VN - lead + k);
+        }
+      });
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (two) {
+      if (by_m) pass(Yes{}, Yes{});
+      else pass(No{}, Yes{});
+    } else {
+      if (by_m) pass(Yes{}, No{});
+      else pass(No{}, No{});
+    }
+    hand_over();
+    z.all = block_sum<NT>(z.all, S);
+    if (by_m) z.enough = block_sum<NT>(z.enough, S);
+    z.before_r = block_sum<NT>(z.before_r, S);
+    if (two) z.before_q = block_sum<NT>(z.before_q, S);
+    if (tid == 0) remote(0).sums[rank] = z;
+    sync_all();
   };
   if (rank != 0) {
     while (true) {
       const Command c = command(Command{});
       if (c.op == kExit) return;
-      collect_bins(c.r0, c.r1, c.q0, c.q1);
+      add_up(c);
     }
   }
 
-  // running sums of the bins
+  // running counts and masses of the bins
   {
-    u64 t = 0, k = 0;
+    u64 k = 0;
+    double m = 0.0, own[kPerBin];
 #pragma unroll
     for (int i = 0; i < kPerBin; ++i) {
-      t += S.tot[kPerBin * tid + i];
-      k += S.tcnt[kPerBin * tid + i];
+      const int b = kPerBin * tid + i;
+      k += S.tcnt[b];
+      own[i] = (double)S.tmass[b] * (exp(step * (double)b) * 0x1p-13);
+      m += own[i];
     }
-    u64 e = block_scan<NT>(t, S), f = by_k ? block_scan<NT>(k, S) : 0;
+    u64 f = block_scan<NT>(k, S);
+    // (in 2^-40 of a largest mass: below 2^19 2^40)
+    double e = (double)block_scan<NT>((u64)(m * 0x1p40), S) * 0x1p-40;
 #pragma unroll
     for (int i = 0; i < kPerBin; ++i) {
-      S.tot[kPerBin * tid + i] = e += S.tot[kPerBin * tid + i];
-      S.tcnt[kPerBin * tid + i] = (uint32_t)(f += S.tcnt[kPerBin * tid + i]);
+      const int b = kPerBin * tid + i;
+      S.tcnt[b] = (uint32_t)(f += S.tcnt[b]);
+      S.est[b] = e += own[i];
     }
     __syncthreads();
   }
-  u64 total = S.tot[kBins - 1], at_least = 0;
-  for (int r = 0; r < C; ++r) at_least += S.kept[r];
-  auto before = [&](int b) -> u64 { return b > 0 ? S.tot[b - 1] : 0ull; };
-  // Collects the tokens of bins r0 .. r1 and q0 .. q1 (r1 < q0, or q1 < q0 for
-  // none) and sorts them; run[] are their running masses in the row. False:
-  // too many.
-  auto gather = [&](int r0, int r1, int q0, int q1) -> bool {
+  // tokens of bins b0 .. b1 (nearly)
+  auto held = [&](int b0, int b1) { return (int)(S.tcnt[b1] - (b0 > 0 ? S.tcnt[b0 - 1] : 0u)); };
+  // The bins where a running mass of `lo` .. `hi`, `mid` most likely, may lie by
+  // the estimates (a token's is off by its rounding, 2^-14, and what the
+  // polynomial leaves, (step / 2)^3 / 6); no more of them than hold `most`
+  // tokens, about the middle (many tokens' errors even out).
+  const double wide = 1.0 + 0x1p-13 - step * step * step / 24.0;
+  auto window = [&](double lo, double mid, double hi, int most, int* b0, int* b1) {
+    const double total = S.est[kBins - 1];
+    int l = first_bin<NT>(S.est, fmin(lo / wide, total), S), h = first_bin<NT>(S.est, fmin(hi * wide, total), S);
+    int m = first_bin<NT>(S.est, fmin(mid, total), S);
+    l = max(l, 0);
+    h = h < 0 ? kBins - 1 : h;
+    m = max(l, min(m < 0 ? kBins - 1 : m, h));
+    if (held(l, h) > most) {
+      const int side = max(0, most - held(m, m)) / 2;
+      const double below = (double)(m > 0 ? S.tcnt[m - 1] : 0u) - side, above = (double)S.tcnt[m] + side + 1.0;
+      if (below > 0.0) l = max(l, first_bin<NT>(S.tcnt, below, S) + 1);
+      const int x = first_bin<NT>(S.tcnt, above, S);
+      if (x > 0) h = min(h, x - 1);
+      l = min(l, m);
+      h = max(h, m);
+    }
+    *b0 = l;
+    *b1 = h;
+  };
+  // Sums and tokens of bins r0 .. r1 and q0 .. q1 (r1 < q0, or q1 < q0 for
+  // none); run[] are the tokens' running masses in the row. False: too many.
+  Sums z;
+  int n_r = 0;
+  auto look = [&](int r0, int r1, int q0, int q1) -> bool {
     __syncthreads();
     if (tid == 0) S.n_list = 0;
     __syncthreads();
-    (void)command(Command{kGather, r0, r1, q0, q1});
-    collect_bins(r0, r1, q0, q1);
+    // The ranges as logits: the smallest of bin < r0, <= r1, < q0 and <= q1 (a bin
+    // never rises with the logit), and the smallest with at least min_p; five
+    // lanes, by bisection over the ordered keys.
+    if (warp == 0) {
+      const int most = lane == 0 ? r0 - 1 : lane == 1 ? r1 : lane == 2 ? q0 - 1 : q1;
+      auto reached = [&](float v) { return lane < 4 ? bin(v) <= most : R.mass(v) >= p.min_p; };
+      uint32_t under = fkey(R.floor) - 1u, upper = fkey(top);  // under: not reached (or no mass); upper: reached
+      const bool any = lane < 4 ? most >= 0 : true;
+      while (__any_sync(0xffffffffu, upper - under > 1u)) {
+        const uint32_t mid = under + (upper - under) / 2u;
+        if (upper - under > 1u) {
+          if (reached(fkey_inv(mid))) upper = mid;
+          else under = mid;
+        }
+      }
+      if (lane < 5) S.ends[lane] = any ? fkey_inv(upper) : INFINITY;
+    }
+    __syncthreads();
+    const Command c = command(Command{kSums, S.ends[0], S.ends[1], q0 <= q1 ? S.ends[2] : INFINITY,
+                                      q0 <= q1 ? S.ends[3] : INFINITY, S.ends[4]});
+    add_up(c);
     n = (int)S.n_list;
+    z = S.sums[0];
+    for (int r = 1; r < C; ++r) {
+      z.all += S.sums[r].all;
+      z.enough += S.sums[r].enough;
+      z.before_r += S.sums[r].before_r;
+      z.before_q += S.sums[r].before_q;
+    }
     if (n > kList) return false;
     sort_list<NT>(n, S);
-    u64 t = 0;
+    u64 t = 0, inside = 0;  // inside: the tokens of r0 .. r1, n_r of them
+    int here = 0;
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
       const int i = kPerList * tid + k;
-      if (i < n) t += R.units_of(Row::value(S.list[i]));
+      if (i < n) {
+        const float v = Row::value(S.list[i]);
+        const u64 w = R.units_of(v);
+        t += w;
+        if (v >= c.rb) {
+          inside += w;
+          ++here;
+        }
+      }
       run[k] = t;
     }
-    const u64 e = block_scan<NT>(t, S) + before(r0);
-    const u64 gap = q0 <= q1 ? before(q0) - S.tot[r1] : 0;
+    const u64 e = block_scan<NT>(t, S);
+    inside = block_sum<NT>(inside, S);
+    n_r = (int)block_sum<NT>((u64)here, S);
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
       const int i = kPerList * tid + k;
-      run[k] += e;
-      if (i < n && q0 <= q1 && bin(Row::value(S.list[i])) >= q0) run[k] += gap;
+      const bool first = i >= n || Row::value(S.list[i]) >= c.rb;
+      run[k] += e + (first ? z.before_r : z.before_q - inside);
     }
     return true;
   };
 
   bool ok = true;
+  u64 total = 0;          // what top-k kept (or all)
+  double total_est = S.est[kBins - 1];
+  bool known = false;     // total is exact
   if (by_k) {
     const int b = first_bin<NT>(S.tcnt, (double)p.top_k, S);
     if (b >= 0) {  // (else all tokens with a mass are kept)
-      ok = gather(b, b, 0, -1);
+      ok = look(b, b, kBins, kBins - 1);
       if (ok) {
         const int i = (int)(p.top_k - 1) - (b > 0 ? (int)S.tcnt[b - 1] : 0);
         __syncthreads();
@@ -863,38 +984,65 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
           if (i == kPerList * tid + k) S.value = run[k];
         __syncthreads();
         total = S.value;
+        total_est = (double)total / kUnit;
+        known = true;
       }
     }
   }
   int i = -1;
-  double M = (double)(by_m && at_least < total ? at_least : total);
-  if (ok && by_p) {
-    const double tp = fmax(1.0, p.top_p * (double)total);
-    const int b = first_bin<NT>(S.tot, tp, S);
-    // the kept mass lies in bin b: so does, mostly, the drawn token's bin
-    const double m0 = fmin(M, fmax(tp, (double)before(b))), m1 = fmin(M, (double)S.tot[b]);
-    const int t0 = first_bin<NT>(S.tot, fmax(1.0, u * m0), S), t1 = first_bin<NT>(S.tot, fmax(1.0, u * m1), S);
-    ok = t1 + 1 >= b ? gather(t0, b, 0, -1) : gather(t0, t1, b, b);
+  double M = 0.0;
+  if (ok) {
+    // the kept mass by estimate, at least and at most; the bins of top-p's
+    // border and of the drawn token
+    double m = total_est, m0 = known ? m : m / wide, m1 = known ? m : m * wide;
+    int q0 = kBins, q1 = kBins - 1, r0, r1;
+    if (by_p) {
+      m *= p.top_p;
+      window(m0 * p.top_p, m, m1 * p.top_p, kList / 2 - 64, &q0, &q1);
+      // (the token at the border is kept whole)
+      m0 = fmax(m0 * p.top_p, q0 > 0 ? S.est[q0 - 1] / wide : 0.0);
+      m1 = fmin(m1, S.est[q1] * wide);
+    }
+    if (by_m) {
+      // the bin where min_p lies
+      const double lb = step < 0.0 ? fmin(log(p.min_p) / step, (double)kBins) : (double)kBins;
+      const int b = min(kBins - 1, (int)lb);
+      m = fmin(m, S.est[b]);
+      m1 = fmin(m1, S.est[min(kBins - 1, b + 1)] * wide);
+      m0 = fmin(m0, b >= 2 ? S.est[b - 2] / wide : 1.0);
+    }
+    window(u * m0, u * m, u * m1, kList / 2 - 64, &r0, &r1);
+    if (q0 <= q1 && r1 + 1 >= q0) {  // one range
+      r0 = min(r0, q0);
+      r1 = max(r1, q1);
+      q0 = kBins;
+      q1 = kBins - 1;
+    }
+    ok = look(r0, r1, q0, q1);
     if (ok) {
-      reach(tp);
-      M = fmin(M, (double)S.value);
-      i = reach(fmax(1.0, u * M));
-    } else {
-      ok = gather(b, b, 0, -1);
+      if (!known) total = z.all;
+      u64 kept = total;
+      if (by_p) {
+        // the border has to lie among the collected tokens of its bins
+        const double tp = fmax(1.0, p.top_p * (double)total);
+        const int at = reach(tp);
+        const int skip = q0 <= q1 ? n_r : 0;
+        ok = at >= skip && (double)(q0 <= q1 ? z.before_q : z.before_r) < tp;
+        if (ok) kept = S.value < kept ? S.value : kept;
+      }
+      if (by_m && z.enough < kept) kept = z.enough;
+      M = (double)kept;
+      const double target = fmax(1.0, u * M);
       if (ok) {
-        reach(tp);
-        M = fmin(M, (double)S.value);
+        i = reach(target);
+        // found among the tokens of r0 .. r1, or, in one range or the other,
+        // right after what comes before it
+        ok = i >= 0 && (double)z.before_r < target;
+        if (ok && q0 <= q1 && i >= n_r) ok = (double)z.before_q < target;
       }
     }
   }
-  if (ok && i < 0) {
-    const double target = fmax(1.0, u * M);
-    const int b = first_bin<NT>(S.tot, target, S);
-    ok = gather(b, b, 0, -1);
-    if (ok) i = reach(target);
-    ok = ok && i >= 0;
-  }
-  (void)command(Command{kExit, 0, 0, 0, 0});
+  (void)command(Command{kExit});
   give(ok ? S.list[i] : draw_slowly<NT>(x, a.V, R, p, u, &M, S), M);
 }
 
