@@ -103,6 +103,12 @@ struct Shared {
   u64 before;
 };
 
+// The exponential's constants (read as operands from constant memory: as
+// immediates each would be moved to two registers for every logit): ln 2 / 512
+// as l, l^2 / 2, l^3 / 6; 1.5 2^52.
+constexpr double kL = 0.0013538030870311431;
+__constant__ double kMassC[4] = {kL, kL * kL / 2.0, kL * kL * kL / 6.0, 6755399441055744.0};
+
 // A row's largest logit and temperature, and the arithmetic of its masses.
 struct Row {
   double top;          // the largest logit
@@ -122,13 +128,13 @@ struct Row {
   // logit that has mass
   __device__ __forceinline__ double mass(float v) const {
     const double d = __dsub_rn((double)v, top);
-    const double kd = __fma_rn(d, scale, 6755399441055744.0);  // + 1.5 2^52: rounded to n
+    const double kd = __fma_rn(d, scale, kMassC[3]);  // + 1.5 2^52: rounded to n
     const int n = __double2loint(kd);
-    const double f = __fma_rn(d, scale, -__dsub_rn(kd, 6755399441055744.0));
-    constexpr double l = 0.0013538030870311431;  // ln 2 / 512
-    const double p = __fma_rn(f, __fma_rn(f, l * l * l / 6.0, l * l / 2.0), l);
+    const double f = __fma_rn(d, scale, -__dsub_rn(kd, kMassC[3]));
+    const double p = __fma_rn(f, __fma_rn(f, kMassC[2], kMassC[1]), kMassC[0]);
     const double t = pow2[n & (kPow2 - 1)];
-    const double s = __hiloint2double(__double2hiint(t) + ((n >> 9) << 20), __double2loint(t));
+    // n / 512 into the exponent: bits 9 and up of n belong at bit 20
+    const double s = __hiloint2double(__double2hiint(t) + ((n & ~(kPow2 - 1)) << 11), __double2loint(t));
     return __fma_rn(s, __dmul_rn(f, p), s);
   }
   // in units of 2^-45: the low bits beside 1.5 2^7, whose last place they are
@@ -137,6 +143,15 @@ struct Row {
   }
   __device__ __forceinline__ u64 units_of(float v) const { return has_mass(v) ? units(mass(v)) : 0ull; }
 };
+
+// acc += m where v >= from (as one predicated addition)
+__device__ __forceinline__ void add_if(double& acc, double m, float v, float from) {
+  asm("{\n\t.reg .pred p;\n\t"
+      "setp.ge.f32 p, %2, %3;\n\t"
+      "@p add.rn.f64 %0, %0, %1;\n\t}"
+      : "+d"(acc)
+      : "d"(m), "f"(v), "f"(from));
+}
 
 template <int NT>
 __device__ u64 block_sum(u64 v, Shared& S) {
@@ -375,9 +390,12 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   const int nvec = (lead + a.V + VN - 1) / VN;
   const int v0 = STREAM ? 0 : rank * vchunk, nv = STREAM ? nvec : max(0, min(vchunk, nvec - v0));
   const uint4* xv = reinterpret_cast<const uint4*>(x - lead) + v0;
+  // whole vectors: [whole0, whole0 + whole_n)
+  const int whole0 = v0 == 0 && lead > 0 ? 1 : 0;
+  const uint32_t whole_n = (uint32_t)max(0, min(nv, (lead + a.V) / VN - v0) - whole0);
   auto load = [&](int i) -> uint4 {
+    if ((uint32_t)(i - whole0) < whole_n) return __ldg(xv + i);
     const int first = (v0 + i) * VN - lead;  // the vector's first logit
-    if (i < nv && first >= 0 && first + VN <= a.V) return __ldg(xv + i);
     union {
       T e[VN];
       uint4 v;
@@ -757,20 +775,25 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     // 2^13 e^(step f) = 2^13 (1 + step f + (step f)^2 / 2), f the distance from
     // the bin's middle in bins, as the low bits beside 2^23
     const float c1 = (float)(8192.0 * step), c2 = (float)(4096.0 * step * step);
-    vectors([&](int, const uint4& q) {
-      if (!R.has_mass(vec_max<T>(q))) return;
-      const Vec<T> e(q);
+    auto pass = [&](auto with_k) {
+      vectors([&](int, const uint4& q) {
+        if (!R.has_mass(vec_max<T>(q))) return;
+        const Vec<T> e(q);
 #pragma unroll
-      for (int k = 0; k < VN; ++k)
-        if (R.has_mass(e.v[k])) {
+        for (int k = 0; k < VN; ++k) {
           const float d = fminf(top - e.v[k], span), b = __fmaf_rn(d, scale, kWhole);
           const float f = __fmaf_rn(d, scale, kWhole - b);
           const float w = __fmaf_rn(f, __fmaf_rn(f, c2, c1), kWhole + 8192.0f);
           const int i = bin_of(b);
-          atomicAdd(&S.bins[0][i], __float_as_uint(w) - 0x4B000000u);
-          if (by_k) atomicAdd(&S.bins[1][i], 1u);
+          if (R.has_mass(e.v[k])) {
+            atomicAdd(&S.bins[0][i], __float_as_uint(w) - 0x4B000000u);
+            if (with_k.value) atomicAdd(&S.bins[1][i], 1u);
+          }
         }
-    });
+      });
+    };
+    if (by_k) pass(std::true_type{});
+    else pass(std::false_type{});
   }
   sync_all();
   // each CTA adds up its share of the bins
@@ -802,18 +825,18 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
         // (192 = 1.5 2^7: its last place is a unit, and a vector's masses do not
         // change its exponent)
         double all = 192.0, before_r = 192.0, before_q = 192.0, enough = 192.0;
-        unsigned hits = 0;
+        bool hit = false;
 #pragma unroll
         for (int k = 0; k < VN; ++k) {
           const float v = e.v[k];
           const double m = R.mass(v);
-          if (R.has_mass(v)) all = __dadd_rn(all, m);
-          if (v >= c.ra) before_r = __dadd_rn(before_r, m);
-          if (with_m.value && v >= c.enough) enough = __dadd_rn(enough, m);
-          if (v >= c.rb && !(v >= c.ra)) hits |= 1u << k;
+          add_if(all, m, v, R.floor);
+          add_if(before_r, m, v, c.ra);
+          if (with_m.value) add_if(enough, m, v, c.enough);
+          hit |= v >= c.rb && v < c.ra;
           if (with_q.value) {
-            if (v >= c.qa) before_q = __dadd_rn(before_q, m);
-            if (v >= c.qb && !(v >= c.qa)) hits |= 1u << k;
+            add_if(before_q, m, v, c.qa);
+            hit |= v >= c.qb && v < c.qa;
           }
         }
         auto units = [](double x) { return (u64)(__double_as_longlong(x) - __double_as_longlong(192.0)); };
@@ -821,10 +844,12 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
         z.before_r += units(before_r);
         if (with_m.value) z.enough += units(enough);
         if (with_q.value) z.before_q += units(before_q);
-        if (hits) {
+        if (hit) {
 #pragma unroll
-          for (int k = 0; k < VN; ++k)
-            if (hits & (1u << k)) put(e.v[k], (v0 + i) * VN - lead + k);
+          for (int k = 0; k < VN; ++k) {
+            const float v = e.v[k];
+            if ((v >= c.rb && v < c.ra) || (with_q.value && v >= c.qb && v < c.qa)) put(v, (v0 + i) * VN - lead + k);
+          }
         }
       });
     };
