@@ -361,8 +361,34 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   uint4* slice = reinterpret_cast<uint4*>(smem + ((sizeof(Shared) + 15) & ~size_t(15)));
   const cg::cluster_group cluster = cg::this_cluster();
   const int C = STREAM ? 1 : (int)cluster.num_blocks(), rank = STREAM ? 0 : (int)cluster.block_rank();
-  const int row = (int)(blockIdx.x / (unsigned)C);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // few candidates: top-k up to half the threads (the quantile of their maxima
+  // is near the k-th largest then), or min-p alone
+  auto kind_of = [&](const nls_draw_params& p) {  // 0: highest logit, 1: few candidates, 2: masses
+    if (p.temperature <= 0.0 || p.min_p > 1.0) return 0;
+    const bool by_k = p.top_k > 0 && p.top_k < a.V;
+    return by_k ? (p.top_k <= NT / 2 ? 1 : 2) : !(p.top_p > 0.0 && p.top_p < 1.0) && p.min_p > 0.0 ? 1 : 2;
+  };
+  int row = (int)(blockIdx.x / (unsigned)C);
+  if constexpr (STREAM) {
+    // Rows that need masses take about three times as long: they come first, so
+    // that they start at once and each on an SM of its own.
+    if (a.rows <= NT) {
+      const bool mine = tid < a.rows && kind_of(a.params[tid]) == 2;
+      const unsigned in_warp = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) S.red[warp] = (u64)__popc(in_warp);
+      __syncthreads();
+      int at = __popc(in_warp & ((1u << lane) - 1u)), all = 0;  // such rows before this one; of all
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        all += (int)S.red[w];
+        if (w < warp) at += (int)S.red[w];
+      }
+      if (tid < a.rows && (mine ? at : all + tid - at) == row) S.pick = tid;
+      __syncthreads();
+      row = S.pick;
+    }
+  }
   auto remote = [&](int r) -> Shared& { return STREAM ? S : *cluster.map_shared_rank(&S, r); };
   auto sync_all = [&] {
     if constexpr (STREAM) __syncthreads();
@@ -375,11 +401,8 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   else asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const nls_draw_params p = a.params[row];
   const double u = a.uniforms ? a.uniforms[row] : -1.0;
-  const bool greedy = p.temperature <= 0.0 || p.min_p > 1.0;
   const bool by_k = p.top_k > 0 && p.top_k < a.V, by_p = p.top_p > 0.0 && p.top_p < 1.0, by_m = p.min_p > 0.0;
-  // few candidates: top-k up to half the threads (the quantile of their maxima
-  // is near the k-th largest then), or min-p alone
-  const bool few = !greedy && ((by_k && p.top_k <= NT / 2) || (!by_k && !by_p && by_m));
+  const bool greedy = kind_of(p) == 0, few = kind_of(p) == 1;
 
   // The row, or the CTA's slice: vectors [v0, v0 + nv), counted from the 16-byte
   // boundary at or before the first logit. Vectors that reach past the row's
@@ -487,6 +510,48 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       cut = f == f ? f - fmaxf(fabsf(f), fabsf(m)) * 0x1p-20f : -INFINITY;
     }
   };
+  // A token's bin: its distance below `ref` in 1023rds of the span, rounded to a
+  // whole number by adding 2^23 (logits below max - 32 T have no mass; those
+  // below the span are in the last bin). The span is finite and not negative,
+  // whatever the temperature, and where the first logits seen are all -inf (low
+  // is +inf then).
+  float ref = 0.0f, span = 0.0f, scale = 0.0f, floor = 0.0f, c1 = 0.0f, c2 = 0.0f;
+  constexpr float kWhole = 8388608.0f;  // 2^23
+  auto bin_of = [](float b) { return (int)min(__float_as_uint(b) - 0x4B000000u, (uint32_t)(kBins - 1)); };
+  auto bin = [&](float v) { return bin_of(__fmaf_rn(fminf(ref - v, span), scale, kWhole)); };
+  // from, to: the span; seen: the largest logit so far (what has no mass beside it
+  // has none beside a larger one)
+  auto set_bins = [&](float from, float to, float seen) {
+    const float widest = fminf((float)(32.5 * p.temperature), 3.402823466e38f);
+    ref = from;
+    span = to <= from ? fminf(from - to, widest) : widest;
+    scale = span > 1e-30f ? (float)(kBins - 1) / span : 0.0f;
+    const double step = scale > 0.0f ? -1.0 / ((double)scale * p.temperature) : 0.0;
+    // 2^13 e^(step f) = 2^13 (1 + step f + (step f)^2 / 2), f the distance from
+    // the bin's middle in bins
+    c1 = (float)(8192.0 * step);
+    c2 = (float)(4096.0 * step * step);
+    floor = Row(seen, p.temperature, nullptr).floor;
+  };
+  auto add_bins = [&](const uint4& q) {
+    if (!(vec_max<T>(q) >= floor)) return;
+    const Vec<T> e(q);
+#pragma unroll
+    for (int k = 0; k < VN; ++k) {
+      const float d = fminf(ref - e.v[k], span), b = __fmaf_rn(d, scale, kWhole);
+      const float f = __fmaf_rn(d, scale, kWhole - b);
+      const float w = __fmaf_rn(f, __fmaf_rn(f, c2, c1), kWhole + 8192.0f);  // (the low bits beside 2^23)
+      const int i = bin_of(b);
+      if (e.v[k] >= floor) {
+        atomicAdd(&S.bins[0][i], __float_as_uint(w) - 0x4B000000u);
+        if (by_k) atomicAdd(&S.bins[1][i], 1u);
+      }
+    }
+  };
+  // A streamed row's first pass fills the bins too, from the largest of its first
+  // logits and a quarter of their span above; a larger one makes a pass of its
+  // own necessary.
+  const bool binned = STREAM && !greedy && !few && p.temperature > 0.0;
   {
     constexpr int U = 4;
     uint4 q[U], nx[U];
@@ -513,6 +578,31 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 #pragma unroll
           for (int k = 0; k < VN; ++k) low = fminf(low, e.v[k] == -INFINITY ? INFINITY : e.v[k]);
         }
+      }
+      if (STREAM && binned) {
+        if (batch == 0) {
+          float m = top, l = low;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
+          }
+          if (lane == 0) {
+            S.fred[0][warp] = m;
+            S.fred[1][warp] = l;
+          }
+          for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            m = fmaxf(m, S.fred[0][w]);
+            l = fminf(l, S.fred[1][w]);
+          }
+          m = fmaxf(m, -3.402823466e38f);
+          set_bins(fminf(m + 0.25f * fminf(m - fminf(l, m), (float)(32.5 * p.temperature)), 3.402823466e38f), l, m);
+        }
+#pragma unroll
+        for (int t = 0; t < U; ++t) add_bins(q[t]);
       }
       if (STREAM && few) {
         // the cut rises as more of the row has been seen
@@ -756,45 +846,15 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 
   // ---- masses of the whole row ------------------------------------------------
   __syncthreads();
-  for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;
-  __syncthreads();
-  // A token's bin: its distance from the largest logit in 1023rds of the span,
-  // rounded to a whole number by adding 2^23 (logits below max - 32 T have no
-  // mass; those below the span are in the last bin). The span is finite and not
-  // negative, whatever the temperature, and where the first logits seen are all
-  // -inf (low is +inf then).
-  const float widest = fminf((float)(32.5 * p.temperature), 3.402823466e38f);
-  const float span = low <= top ? fminf(top - low, widest) : widest;
-  const float scale = span > 1e-30f ? (float)(kBins - 1) / span : 0.0f;
-  constexpr float kWhole = 8388608.0f;  // 2^23
-  auto bin_of = [](float b) { return (int)min(__float_as_uint(b) - 0x4B000000u, (uint32_t)(kBins - 1)); };
-  auto bin = [&](float v) { return bin_of(__fmaf_rn(fminf(top - v, span), scale, kWhole)); };
-  // ln(mass) per bin
-  const double step = scale > 0.0f ? -1.0 / ((double)scale * p.temperature) : 0.0;
-  {
-    // 2^13 e^(step f) = 2^13 (1 + step f + (step f)^2 / 2), f the distance from
-    // the bin's middle in bins, as the low bits beside 2^23
-    const float c1 = (float)(8192.0 * step), c2 = (float)(4096.0 * step * step);
-    auto pass = [&](auto with_k) {
-      vectors([&](int, const uint4& q) {
-        if (!R.has_mass(vec_max<T>(q))) return;
-        const Vec<T> e(q);
-#pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const float d = fminf(top - e.v[k], span), b = __fmaf_rn(d, scale, kWhole);
-          const float f = __fmaf_rn(d, scale, kWhole - b);
-          const float w = __fmaf_rn(f, __fmaf_rn(f, c2, c1), kWhole + 8192.0f);
-          const int i = bin_of(b);
-          if (R.has_mass(e.v[k])) {
-            atomicAdd(&S.bins[0][i], __float_as_uint(w) - 0x4B000000u);
-            if (with_k.value) atomicAdd(&S.bins[1][i], 1u);
-          }
-        }
-      });
-    };
-    if (by_k) pass(std::true_type{});
-    else pass(std::false_type{});
+  if (!binned || !(top <= ref)) {
+    set_bins(top, low, top);
+    for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;
+    __syncthreads();
+    vectors([&](int, const uint4& q) { add_bins(q); });
   }
+  // ln(mass) per bin, and the bins' zero from the largest logit
+  const double step = scale > 0.0f ? -1.0 / ((double)scale * p.temperature) : 0.0;
+  const double zero = ((double)ref - (double)top) / p.temperature;
   sync_all();
   // each CTA adds up its share of the bins
   {
@@ -886,7 +946,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     for (int i = 0; i < kPerBin; ++i) {
       const int b = kPerBin * tid + i;
       k += S.tcnt[b];
-      own[i] = (double)S.tmass[b] * (exp(step * (double)b) * 0x1p-13);
+      own[i] = (double)S.tmass[b] * (exp(fmin(step * (double)b + zero, 40.0)) * 0x1p-13);
       m += own[i];
     }
     u64 f = block_scan<NT>(k, S);
@@ -941,7 +1001,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       const int most = lane == 0 ? r0 - 1 : lane == 1 ? r1 : lane == 2 ? q0 - 1 : q1;
       auto reached = [&](float v) { return lane < 4 ? bin(v) <= most : R.mass(v) >= p.min_p; };
       uint32_t under = fkey(R.floor) - 1u, upper = fkey(top);  // under: not reached (or no mass); upper: reached
-      const bool any = lane < 4 ? most >= 0 : true;
+      const bool any = lane < 4 ? bin(top) <= most : true;  // (else no logit is)
       while (__any_sync(0xffffffffu, upper - under > 1u)) {
         const uint32_t mid = under + (upper - under) / 2u;
         if (upper - under > 1u) {
@@ -1003,6 +1063,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       ok = look(b, b, kBins, kBins - 1);
       if (ok) {
         const int i = (int)(p.top_k - 1) - (b > 0 ? (int)S.tcnt[b - 1] : 0);
+        ok = i < n;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kPerList; ++k)
@@ -1030,7 +1091,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
     if (by_m) {
       // the bin where min_p lies
-      const double lb = step < 0.0 ? fmin(log(p.min_p) / step, (double)kBins) : (double)kBins;
+      const double lb = step < 0.0 ? fmax(0.0, fmin((log(p.min_p) - zero) / step, (double)kBins)) : (double)kBins;
       const int b = min(kBins - 1, (int)lb);
       m = fmin(m, S.est[b]);
       m1 = fmin(m1, S.est[min(kBins - 1, b + 1)] * wide);
