@@ -881,34 +881,49 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     auto pass = [&](auto with_m, auto with_q) {
       vectors([&](int i, const uint4& q) {
         if (!__any_sync(0xffffffffu, R.has_mass(vec_max<T>(q)))) return;
-        const Vec<T> e(q);
-        // (192 = 1.5 2^7: its last place is a unit, and a vector's masses do not
-        // change its exponent)
-        double all = 192.0, before_r = 192.0, before_q = 192.0, enough = 192.0;
-        bool hit = false;
+        // four logits at a time (eight would not fit the registers); 192 = 1.5
+        // 2^7: its last place is a unit, and their masses do not change its
+        // exponent
+#pragma unroll 1
+        for (int g = 0; g < VN; g += 4) {
+          float e[4];
+          if constexpr (VN == 4) {
+            e[0] = __uint_as_float(q.x);
+            e[1] = __uint_as_float(q.y);
+            e[2] = __uint_as_float(q.z);
+            e[3] = __uint_as_float(q.w);
+          } else {
+            const Vec<T> both(g == 0 ? make_uint4(q.x, q.y, 0u, 0u) : make_uint4(q.z, q.w, 0u, 0u));
 #pragma unroll
-        for (int k = 0; k < VN; ++k) {
-          const float v = e.v[k];
-          const double m = R.mass(v);
-          add_if(all, m, v, R.floor);
-          add_if(before_r, m, v, c.ra);
-          if (with_m.value) add_if(enough, m, v, c.enough);
-          hit |= v >= c.rb && v < c.ra;
-          if (with_q.value) {
-            add_if(before_q, m, v, c.qa);
-            hit |= v >= c.qb && v < c.qa;
+            for (int k = 0; k < 4; ++k) e[k] = both.v[k];
           }
-        }
-        auto units = [](double x) { return (u64)(__double_as_longlong(x) - __double_as_longlong(192.0)); };
-        z.all += units(all);
-        z.before_r += units(before_r);
-        if (with_m.value) z.enough += units(enough);
-        if (with_q.value) z.before_q += units(before_q);
-        if (hit) {
+          double all = 192.0, before_r = 192.0, before_q = 192.0, enough = 192.0;
+          bool hit = false;
 #pragma unroll
-          for (int k = 0; k < VN; ++k) {
-            const float v = e.v[k];
-            if ((v >= c.rb && v < c.ra) || (with_q.value && v >= c.qb && v < c.qa)) put(v, (v0 + i) * VN - lead + k);
+          for (int k = 0; k < 4; ++k) {
+            const float v = e[k];
+            const double m = R.mass(v);
+            add_if(all, m, v, R.floor);
+            add_if(before_r, m, v, c.ra);
+            if (with_m.value) add_if(enough, m, v, c.enough);
+            hit |= v >= c.rb && v < c.ra;
+            if (with_q.value) {
+              add_if(before_q, m, v, c.qa);
+              hit |= v >= c.qb && v < c.qa;
+            }
+          }
+          auto units = [](double x) { return (u64)(__double_as_longlong(x) - __double_as_longlong(192.0)); };
+          z.all += units(all);
+          z.before_r += units(before_r);
+          if (with_m.value) z.enough += units(enough);
+          if (with_q.value) z.before_q += units(before_q);
+          if (hit) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float v = e[k];
+              if ((v >= c.rb && v < c.ra) || (with_q.value && v >= c.qb && v < c.qa))
+                put(v, (v0 + i) * VN - lead + g + k);
+            }
           }
         }
       });

@@ -52,6 +52,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -70,6 +71,7 @@ constexpr int kStep = 2 * kHalf;  // columns per step
 constexpr int kRawBytes = kTile * kStep / 2;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxSmem = 227 * 1024;
 
 enum class Op { kI8, kF16, kBF16 };
 // Tensor memory: a half step's operand takes 32 (bytes) or 64 columns per tile
@@ -952,6 +954,29 @@ EncodeTiledFn encode_tiled() {
 }
 
 
+// The kernels' dynamic shared memory limit, raised once per device to the most
+// there is (the attribute call costs host time on every launch otherwise).
+cudaError_t allow_smem(const void* kern, int bytes) {
+  struct Seen {
+    std::atomic<const void*> kern{nullptr};
+    std::atomic<uint64_t> devices{0};
+  };
+  static Seen seen[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  for (Seen& k : seen) {
+    const void* none = nullptr;
+    if (k.kern.load(std::memory_order_acquire) != kern && !k.kern.compare_exchange_strong(none, kern) && none != kern)
+      continue;
+    if (dev < 64 && (k.devices.load(std::memory_order_acquire) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (e == cudaSuccess && dev < 64) k.devices.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+  }
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 template <Op OP, int R>
 const void* kernel_of(int nbt) {
   if constexpr (OP == Op::kI8) {
@@ -1038,7 +1063,7 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     k.s_off = k.x_off + 2 * half_bytes;
     k.m_off = k.s_off + 2 * p.regions * kTile * k.ssize;
     k.stage_bytes = (k.m_off + (a.mins ? 2 * p.regions * kTile * k.ssize : 0) + 1023) & ~1023;
-    const int room = 227 * 1024 - 1024 - (int)sizeof(Bars);
+    const int room = kMaxSmem - 1024 - (int)sizeof(Bars);
     k.stages = std::min(kMaxStages, room / k.stage_bytes);
     const size_t smem = (size_t)k.stages * k.stage_bytes + sizeof(Bars);
     const void* kern = i8 ? kernel_of<Op::kI8>(p.regions, w.nbt)
@@ -1061,7 +1086,7 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     b0 += w.nb;
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    e = allow_smem(kern, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, 1, 1);

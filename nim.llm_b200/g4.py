@@ -10,7 +10,6 @@ to it.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import numpy as np
@@ -18,12 +17,18 @@ import numpy as np
 from ._abi import DRAW_PARAMS_DTYPE, G4WeightsStruct, NLS_DT
 
 
+_DT_CODES: dict = {}   # torch dtype -> NLS_DT_*
+
+
 def dt_code(dtype) -> int:
     """NLS_DT_* of a torch dtype."""
-    name = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}.get(str(dtype))
-    if name is None:
-        raise TypeError(f"float32, float16 or bfloat16 expected, not {dtype}")
-    return NLS_DT[name]
+    code = _DT_CODES.get(dtype)
+    if code is None:
+        name = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16"}.get(str(dtype))
+        if name is None:
+            raise TypeError(f"float32, float16 or bfloat16 expected, not {dtype}")
+        code = _DT_CODES[dtype] = NLS_DT[name]
+    return code
 
 
 def _line(rows: int) -> int:
@@ -40,43 +45,42 @@ class G4Weights:
 
     def __init__(self, q, scales, mins=None, group: int = 128):
         import torch
-        if q.dim() != 2 or q.dtype != torch.uint8 or q.stride(1) != 1:
+        if q.dtype != torch.uint8 or q.dim() != 2 or q.stride(1) != 1:
             raise ValueError("q must be a uint8 matrix with contiguous rows")
-        rows, cols = q.shape[0], 2 * q.shape[1]
+        rows, cols = q.shape
+        cols *= 2
         group = int(group)
         if group not in (32, 64) and (group < 128 or group % 128):
             raise ValueError("group must be 32, 64 or a multiple of 128")
         if rows < 1 or cols < 32 or cols % 32:
             raise ValueError("at least one row, and columns in whole 32, are needed")
+        lines = -(-cols // group)
+        s_ld = scales.stride(0) if lines > 1 else _line(rows)
+        q_ld = q.stride(0) if rows > 1 else -(-cols // 32) * 16
+        if q_ld % 16 or s_ld % 8 or s_ld < rows:
+            raise ValueError("q's rows must be 16-byte multiples apart and the scales' lines multiples of 8 values")
+        dtype, device = scales.dtype, q.device
         for name, t in (("scales", scales), ("mins", mins)):
             if t is None:
                 continue
-            if tuple(t.shape) != (-(-cols // group), rows) or t.stride(1) != 1:
-                raise ValueError(f"{name} must be [ceil(cols / group), rows] with contiguous lines")
-            if t.device != q.device or t.dtype != scales.dtype:
+            if tuple(t.shape) != (lines, rows) or t.stride(1) != 1 or (lines > 1 and t.stride(0) != s_ld):
+                raise ValueError(f"{name} must be [ceil(cols / group), rows] with contiguous lines, scales and mins "
+                                 "with the same line stride")
+            if t.device != device or t.dtype != dtype:
                 raise ValueError(f"{name} must be on q's device and of the scales' type")
-        lines = scales.shape[0]
-        s_ld = scales.stride(0) if lines > 1 else _line(rows)
-        if mins is not None and lines > 1 and mins.stride(0) != s_ld:
-            raise ValueError("scales and mins must have the same line stride")
-        q_ld = q.stride(0) if rows > 1 else -(-(cols // 2) // 16) * 16
-        if q_ld % 16 or s_ld % 8 or s_ld < rows:
-            raise ValueError("q's rows must be 16-byte multiples apart and the scales' lines multiples of 8 values")
-        # the library reads a line in whole 16-byte pieces: the last one too
-        # needs the room behind its last value
-        for t in (scales, mins):
-            if t is not None and t.untyped_storage().nbytes() < \
+            # the library reads a line in whole 16-byte pieces: the last one too
+            # needs the room behind its last value
+            if rows % 8 and t.untyped_storage().nbytes() < \
                     (t.storage_offset() + (lines - 1) * s_ld + _line(rows)) * t.element_size():
                 raise ValueError("the last line of scales needs room for rows rounded up to 8 values (g4_pack makes it)")
-        for t in (q, scales, mins):
-            if t is not None and t.data_ptr() % 16:
-                raise ValueError("q, scales and mins must be 16-byte aligned")
+        qp, sp = q.data_ptr(), scales.data_ptr()
+        mp = None if mins is None else mins.data_ptr()
+        if (qp | sp | (mp or 0)) % 16:
+            raise ValueError("q, scales and mins must be 16-byte aligned")
         self.q, self.scales, self.mins = q, scales, mins
         self.rows, self.cols, self.group = rows, cols, group
-        self.device = q.device
-        self.struct = G4WeightsStruct(q.data_ptr(), scales.data_ptr(),
-                                      None if mins is None else mins.data_ptr(), q_ld, s_ld, rows, cols,
-                                      group, dt_code(scales.dtype))
+        self.device = device
+        self.struct = G4WeightsStruct(qp, sp, mp, q_ld, s_ld, rows, cols, group, dt_code(dtype))
 
     def __repr__(self) -> str:
         return (f"G4Weights({self.rows} x {self.cols}, group={self.group}, {self.scales.dtype}"
@@ -152,9 +156,10 @@ def draw_params(rows: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> np
 def rows_of(t, device_index: Optional[int], what: str):
     """(pointer, values from row to row) of a 2-d tensor with contiguous rows
     on the engine's device (None: host memory)."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
         raise ValueError(f"{what}: a matrix with contiguous rows expected")
     if t.device.index != device_index:
         raise ValueError(f"{what} is on {t.device}, " + ("other arguments on the host" if device_index is None else
                                                           f"the engine on cuda:{device_index}"))
-    return ctypes.c_void_p(t.data_ptr()), (t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1]))
+    return t.data_ptr(), (stride[0] if shape[0] > 1 else max(1, shape[1]))

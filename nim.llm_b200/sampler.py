@@ -99,6 +99,7 @@ class Engine:
         self.device = device
         self.max_rows = max_rows
         self.max_vocab = max_vocab
+        self._torch_device = None
 
     def close(self):
         if getattr(self, "_h", None):
@@ -340,17 +341,17 @@ class Engine:
         given stream (None: torch's current one), on which temporaries are made
         and results allocated."""
         if not cuda:
-            return contextlib.nullcontext()
+            return _NO_CONTEXT
         import torch
-        dev = torch.device("cuda", self.device)
-        return torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else
-                                 torch.cuda.ExternalStream(int(stream), device=dev))
+        if stream is None:
+            return _NO_CONTEXT if torch.cuda.current_device() == self.device else torch.cuda.device(self.device)
+        return torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", self.device)))
 
     def _stream(self, cuda: bool, stream):
-        if not cuda:
-            return ctypes.c_void_p(0 if stream is None else int(stream))
+        if not cuda or stream is not None:
+            return 0 if stream is None else int(stream)
         import torch
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return torch.cuda.current_stream(self.device).cuda_stream
 
     def _finish(self, st: int, what: str, cuda: bool, stream, check: bool) -> int:
         """Raise on a call's error. Arguments and launches are always checked;
@@ -424,7 +425,9 @@ class Engine:
                     raise ValueError(f"{what}: {B} contiguous {np.dtype(dt).name} expected")
             return (params, uniforms, ids, probs, _host_ptr(params), _host_ptr(uniforms), _host_ptr(ids),
                     _host_ptr(probs))
-        dev = torch.device("cuda", self.device)
+        dev = self._torch_device
+        if dev is None:
+            dev = self._torch_device = torch.device("cuda", self.device)
         if not _is_torch(params):
             params = torch.from_numpy(np.ascontiguousarray(params, dtype=DRAW_PARAMS_DTYPE).view(np.uint8)).to(dev)
         if uniforms is not None and not _is_torch(uniforms):
@@ -437,8 +440,8 @@ class Engine:
                             (probs, torch.float32, "out_probs")):
             if t is not None and (t.device != dev or t.dtype != dt or not t.is_contiguous() or t.numel() != B):
                 raise ValueError(f"{what}: {B} contiguous {dt} on {dev} expected")
-        ptr = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
-        return params, uniforms, ids, probs, ptr(params), ptr(uniforms), ptr(ids), ptr(probs)
+        return (params, uniforms, ids, probs, params.data_ptr(), None if uniforms is None else uniforms.data_ptr(),
+                ids.data_ptr(), probs.data_ptr())
 
     def draw_batch(self, logits, params, uniforms=None, out_ids=None, out_probs=None, stream=None,
                    check: bool = True):
@@ -501,6 +504,8 @@ class Engine:
         self._check(st, "nls_argmax_batch")
         return ids
 
+
+_NO_CONTEXT = contextlib.nullcontext()
 
 _default_engine: Optional[Engine] = None
 
