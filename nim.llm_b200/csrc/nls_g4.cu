@@ -107,9 +107,11 @@ __host__ __device__ constexpr int mma_n(Op op, int nbt) {
 // 4096).
 __host__ __device__ constexpr int i8_rows(int regions) { return regions == 4 ? 4 : 12; }
 // bytes of a half step's laid-out activations: bytes (and per region and batch
-// row four words for the joining), or 16-bit parts
+// row four words for the joining), or 16-bit parts (and per region and column
+// their sum)
 __host__ __device__ constexpr int x_half(Op op, int nbt, int regions, int parts) {
-  return op == Op::kI8 ? mma_n(op, nbt) * kHalf + regions * nbt * 16 : parts * mma_n(op, nbt) * kHalf * 2;
+  return op == Op::kI8 ? mma_n(op, nbt) * kHalf + regions * nbt * 16
+                       : mma_n(op, nbt) * (parts * kHalf * 2 + regions * 4);
 }
 
 // How a launch of nb batch rows goes.
@@ -135,8 +137,8 @@ struct Plan {
   int ksteps, tiles, grid, regions;
   int64_t steps;  // tiles * ksteps
   // workspace
-  size_t x_bytes, sum_bytes, part_bytes, count_bytes;
-  size_t total() const { return x_bytes + sum_bytes + part_bytes + count_bytes; }
+  size_t x_bytes, part_bytes, count_bytes;
+  size_t total() const { return x_bytes + part_bytes + count_bytes; }
 };
 
 Plan plan_of(const G4Args& a, int sm_count) {
@@ -150,7 +152,6 @@ Plan plan_of(const G4Args& a, int sm_count) {
     const Way w = way_of(a, a.nb - b0);
     const size_t halves = (size_t)p.ksteps * 2;
     p.x_bytes = std::max(p.x_bytes, (halves * x_half(w.op, w.nbt, p.regions, w.parts) + 255) & ~size_t(255));
-    if (a.mins && w.op != Op::kI8) p.sum_bytes = std::max(p.sum_bytes, halves * p.regions * w.n * sizeof(float));
     p.part_bytes = std::max(p.part_bytes, (size_t)p.grid * 2 * w.nbt * kTile * sizeof(float));
     b0 += w.nb;
     if (a.nb - b0 > 2 * 64) b0 = a.nb - 64 - (a.nb - b0) % 64;  // (passes in between are all alike)
@@ -167,7 +168,6 @@ struct KernelArgs {
   int lines;            // lines of scales as the halves use them: of whole groups up to 128 wide, else per half
   int nb;
   const uint8_t* x;     // laid-out activations, x_half bytes per half step
-  const float* xsum;    // their sums [half step][regions][N] (floating point with minimums)
   float* part;          // partial tiles [2 * grid][NB][256]
   int* count;           // steps joined so far, per tile
   void* y;
@@ -280,12 +280,12 @@ __global__ void __launch_bounds__(512) g4_bytes_kernel(const X* x, int64_t ldx, 
 // The floating-point way. One block per half step; a thread takes 8 columns of a batch row and writes them,
 // permuted, as one 16-byte line of the operand (no-swizzle K-major: 8 rows x 16
 // bytes per core matrix, K step j of 16 columns at j * N * 32), for each part.
-// With minimums it also sums them per region (the 16 threads of a batch row
+// Behind the operand come their sums per region (the 16 threads of a batch row
 // are neighbours). Rows nb .. N - 1 and columns past the matrix are zeros.
 template <class X>
 __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx, int nb, int n_cols, int cols,
-                                                         int parts, int regions, uint8_t* op, float* xsum,
-                                                         int* count, int tiles, int* status, int clear_status) {
+                                                         int parts, int regions, uint8_t* op, int half_bytes, int* count,
+                                                          int tiles, int* status, int clear_status) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   clear_counts(count, tiles, status, clear_status);
   const int k = blockIdx.x, n = threadIdx.x >> 4, word = threadIdx.x & 15;
@@ -295,15 +295,16 @@ __global__ void __launch_bounds__(1024) g4_layout_kernel(const X* x, int64_t ldx
   load8(x, ldx, nb, cols, n, k * kHalf + word * 8, v);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] *= kIn;
-  if (xsum) {
+  uint8_t* half = op + (size_t)k * half_bytes;
+  {
     float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     const int lanes = 16 / regions;
     for (int o = 1; o < lanes; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (word % lanes == 0) xsum[((size_t)k * regions + word / lanes) * n_cols + n] = s;
+    if (word % lanes == 0)
+      reinterpret_cast<float*>(half + parts * n_cols * (kHalf * 2))[(word / lanes) * n_cols + n] = s;
   }
   constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-  uint8_t* dst = op + (size_t)k * parts * n_cols * (kHalf * 2) + (size_t)(word >> 1) * (n_cols * 32) +
-                 (n >> 3) * 256 + (word & 1) * 128 + (n & 7) * 16;
+  uint8_t* dst = half + (size_t)(word >> 1) * (n_cols * 32) + (n >> 3) * 256 + (word & 1) * 128 + (n & 7) * 16;
 #pragma unroll
   for (int part = 0; part < (kF32 ? 3 : 1); ++part) {
     uint32_t w[4];
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(threads_of(OP, NB), 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tbase = B.tmem;
-  // the laid-out activations, their sums and the cleared counters are there
+  // the laid-out activations and the cleared counters are there
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // (a limit of 0 is a deadline already past: every role but the copies, whose
@@ -821,15 +822,20 @@ __global__ void __launch_bounds__(threads_of(OP, NB), 1)
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         if (!I8 && a.mins) {
 #pragma unroll
-          for (int h = 0; h < kTogether; ++h)
+          for (int h = 0; h < kTogether; ++h) {
+            const float* xs = reinterpret_cast<const float*>(st + a.x_off + (h0 + h) * x_half(OP, NB, R, a.parts) +
+                                                             a.parts * (N * kHalf * 2)) + b0;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-              const int l = (2 * k + h0 + h) * R + r;
-              if (l >= a.lines) break;
-              const float* xs = a.xsum + (size_t)l * N + b0;
+            for (int r = 0; r < R; ++r)  // (past the matrix: zero times a sum of zeros)
 #pragma unroll
-              for (int j = 0; j < CB; ++j) acc[j] = __fmaf_rn(mn[h][r], xs[j], acc[j]);
-            }
+              for (int j = 0; j < CB; j += 4) {
+                const float4 x4 = *reinterpret_cast<const float4*>(xs + r * N + j);
+                acc[j] = __fmaf_rn(mn[h][r], x4.x, acc[j]);
+                acc[j + 1] = __fmaf_rn(mn[h][r], x4.y, acc[j + 1]);
+                acc[j + 2] = __fmaf_rn(mn[h][r], x4.z, acc[j + 2]);
+                acc[j + 3] = __fmaf_rn(mn[h][r], x4.w, acc[j + 3]);
+              }
+          }
         }
         __syncwarp();
         if (lane == 0) {
@@ -1040,9 +1046,8 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
   k.stype = a.stype;
   k.ssize = (int)dt_size(a.stype);
   k.x = ws;
-  float* xsum = reinterpret_cast<float*>(ws + p.x_bytes);
-  k.part = reinterpret_cast<float*>(ws + p.x_bytes + p.sum_bytes);
-  k.count = reinterpret_cast<int*>(ws + p.x_bytes + p.sum_bytes + p.part_bytes);
+  k.part = reinterpret_cast<float*>(ws + p.x_bytes);
+  k.count = reinterpret_cast<int*>(ws + p.x_bytes + p.part_bytes);
   k.ytype = a.ytype;
   k.ldy = a.ldy;
   k.ksteps = p.ksteps;
@@ -1056,7 +1061,6 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
     const int half_bytes = x_half(w.op, w.nbt, p.regions, w.parts);
     k.nb = w.nb;
     k.parts = w.parts;
-    k.xsum = a.mins && !i8 ? xsum : nullptr;
     k.out_scale = w.op == Op::kBF16 ? 4096.0f : 1.0f;
     k.y = static_cast<uint8_t*>(a.y) + (size_t)b0 * a.ldy * yes;
     k.x_off = kRawBytes;
@@ -1080,8 +1084,8 @@ cudaError_t launch_g4(const G4Args& a, void* workspace, int sm_count, cudaStream
                                                              clear);
       else
         g4_layout_kernel<X><<<2 * p.ksteps, 16 * w.n, 0, st>>>(static_cast<const X*>(x), a.ldx, w.nb, w.n, a.cols,
-                                                               w.parts, p.regions, ws, const_cast<float*>(k.xsum),
-                                                               k.count, p.tiles, a.status, clear);
+                                                               w.parts, p.regions, ws, half_bytes, k.count, p.tiles,
+                                                               a.status, clear);
     });
     b0 += w.nb;
     cudaError_t e = cudaGetLastError();
