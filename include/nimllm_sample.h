@@ -368,8 +368,8 @@ typedef struct nls_g4_weights {
   const void* mins;   /* as scales, or NULL */
   int64_t q_ld;       /* bytes from a row of q to the next: a multiple of 16, >= cols / 2 */
   int64_t s_ld;       /* values from a group's line to the next: a multiple of 8, >= rows */
-  int32_t rows;
-  int32_t cols;       /* a multiple of 32 */
+  int32_t rows;       /* at most 2^30 */
+  int32_t cols;       /* a multiple of 32, at most 2^24 */
   int32_t group;      /* 32, 64 or a multiple of 128; the last group may be short */
   int32_t stype;      /* type of scales and mins: NLS_DT_* */
 } nls_g4_weights;

@@ -665,6 +665,8 @@ bool g4_weights_ok(const nls_g4_weights* w) {
   if (!w || !w->q || !w->scales) return false;
   if (!aligned_to(w->q, 16) || !aligned_to(w->scales, 16) || !aligned_to(w->mins, 16)) return false;
   if (w->rows < 1 || w->cols < 32 || w->cols % 32 != 0 || !nls::dt_ok(w->stype)) return false;
+  // (the kernels count rows, columns and threads in 32 bits)
+  if (w->rows > 1 << 30 || w->cols > 1 << 24) return false;
   if (w->group != 32 && w->group != 64 && (w->group < 128 || w->group % 128 != 0)) return false;
   return w->q_ld % 16 == 0 && w->q_ld >= w->cols / 2 && w->s_ld % 8 == 0 && w->s_ld >= w->rows;
 }

@@ -54,6 +54,8 @@ class G4Weights:
             raise ValueError("group must be 32, 64 or a multiple of 128")
         if rows < 1 or cols < 32 or cols % 32:
             raise ValueError("at least one row, and columns in whole 32, are needed")
+        if rows > 1 << 30 or cols > 1 << 24:
+            raise ValueError("at most 2^30 rows and 2^24 columns")
         lines = -(-cols // group)
         s_ld = scales.stride(0) if lines > 1 else _line(rows)
         q_ld = q.stride(0) if rows > 1 else -(-cols // 32) * 16

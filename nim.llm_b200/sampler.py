@@ -345,7 +345,10 @@ class Engine:
         import torch
         if stream is None:
             return _NO_CONTEXT if torch.cuda.current_device() == self.device else torch.cuda.device(self.device)
-        return torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", self.device)))
+        device = torch.device("cuda", self.device)
+        if int(stream) == 0:  # (an external stream of handle 0 would be a new one)
+            return torch.cuda.stream(torch.cuda.default_stream(device))
+        return torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device))
 
     def _stream(self, cuda: bool, stream):
         if not cuda or stream is not None:

@@ -339,6 +339,38 @@ def test_device_refusals(pkg, eng):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("big", [dict(cols=2**24 + 32), dict(cols=2**28), dict(cols=2**31 - 32), dict(rows=2**30 + 1),
+                                 dict(rows=2**31 - 1)])
+def test_sizes_past_the_range_are_refused(pkg, eng, big):
+    import torch
+    w = make(pkg, 64, 128, 32, "f16", True)
+    s = pkg._abi.G4WeightsStruct.from_buffer_copy(w.struct)
+    s.q_ld, s.s_ld = 2**31, 2**31
+    for k, v in big.items():
+        setattr(s, k, v)
+    x = torch.zeros(128, device="cuda")
+    assert pkg.load().nls_g4_matmul(eng._h, ctypes.byref(s), x.data_ptr(), 0, 2**31, 1, x.data_ptr(), 0, 2**31, 3, None) == 1
+
+
+@pytest.mark.gpu
+def test_the_default_stream_by_its_handle(pkg, eng):
+    """stream=0 is the default stream, for temporaries and results too."""
+    import torch
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        with eng._on(True, 0):
+            assert torch.cuda.current_stream() == torch.cuda.default_stream()
+        with eng._on(True, side.cuda_stream):
+            assert torch.cuda.current_stream().cuda_stream == side.cuda_stream
+    w = make(pkg, 300, 256, 64, "f16", False)
+    x = torch.randn((256, 3), device="cuda").t()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        y = eng.g4_matmul(w, x, stream=0)
+    assert torch.equal(y, eng.g4_matmul(w, x))
+
+
+@pytest.mark.gpu
 def test_capture_that_would_have_to_allocate(pkg, eng):
     """Refused, and the capture goes on."""
     import torch
