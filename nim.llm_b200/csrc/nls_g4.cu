@@ -798,6 +798,14 @@ __global__ void __launch_bounds__(threads_of(OP, NB), 1)
             for (int r = 0; r < R; ++r)
               tmem_ld<C * (I8 ? 4 : 1)>(td + (uint32_t)((buf.i + h) * (2 * R * N) + r * N + c * (I8 ? 4 : 1)), d[h][r]);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (c + C >= CB) {  // all sums are in registers: the MMAs may have their place
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+              for (int h = 0; h < kTogether; ++h) arrive(added0 + (uint32_t)(buf.i + h) * 8);
+            }
+          }
 #pragma unroll
           for (int h = 0; h < kTogether; ++h)
 #pragma unroll
@@ -819,7 +827,6 @@ __global__ void __launch_bounds__(threads_of(OP, NB), 1)
                 }
               }
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         if (!I8 && a.mins) {
 #pragma unroll
           for (int h = 0; h < kTogether; ++h) {
@@ -837,11 +844,9 @@ __global__ void __launch_bounds__(threads_of(OP, NB), 1)
               }
           }
         }
-        __syncwarp();
-        if (lane == 0) {
-#pragma unroll
-          for (int h = 0; h < kTogether; ++h) arrive(added0 + (uint32_t)(buf.i + h) * 8);
-          if (h0 + kTogether == 2) arrive(free0 + (uint32_t)slot.i * 8);
+        if (h0 + kTogether == 2) {
+          __syncwarp();
+          if (lane == 0) arrive(free0 + (uint32_t)slot.i * 8);
         }
         buf.next(kBuffers, kTogether);
       }
