@@ -89,7 +89,7 @@ struct Shared {
     u64 tot[kBins];       // radix selection
   };
   double pow2[kPow2];  // 2^(j / 512)
-  u64 red[kMaxWarps];
+  u64 red[kMaxWarps], reds[4][kMaxWarps];
   u64 first[kMaxCluster];  // each CTA's first highest logit
   Sums sums[kMaxCluster];
   float top[kMaxCluster], low[kMaxCluster];
@@ -97,7 +97,7 @@ struct Shared {
   Command cmd;
   float ends[5];
   unsigned n_list, n_mine;
-  int pick;
+  int pick, picks[3];
   u64 value;
   u64 lo;              // radix selection
   u64 before;
@@ -197,35 +197,97 @@ __device__ int first_bin(const V* run, double target, Shared& S) {
   return S.pick;
 }
 
-// S.list[0 .. n) ascending (n <= kList)
+// first_bin of three targets
+template <int NT>
+__device__ void first_bins(const double* run, const double (&target)[3], int (&bin)[3], Shared& S) {
+  __syncthreads();
+  if (threadIdx.x < 3) S.picks[threadIdx.x] = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += NT) {
+    const double at = run[b], before = b > 0 ? run[b - 1] : -1.0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (at >= target[k] && (b == 0 || before < target[k])) S.picks[k] = b;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) bin[k] = S.picks[k];
+}
+
+// S.list[0 .. n) ascending (n <= kList): bitonic. A warp keeps 64 neighbours in
+// registers for the strides below 64; larger strides go through shared memory,
+// two at a time. (Few barriers: with one stride each, 555 tokens took 17000
+// cycles.)
 template <int NT>
 __device__ void sort_list(int n, Shared& S) {
-  int p = 32;
+  const int lane = threadIdx.x & 31;
+  int p = 64;
   while (p < n) p <<= 1;
   for (int i = n + (int)threadIdx.x; i < p; i += NT) S.list[i] = ~0ull;
   __syncthreads();
-  for (int size = 2; size <= p; size <<= 1) {
-    for (int stride = size >> 1; stride >= 32; stride >>= 1) {
-      for (int i = threadIdx.x; i < p / 2; i += NT) {
-        const int a = ((i & ~(stride - 1)) << 1) | (i & (stride - 1)), b = a + stride;
-        const u64 x = S.list[a], y = S.list[b];
-        if ((x > y) == ((a & size) == 0)) {
-          S.list[a] = y;
-          S.list[b] = x;
-        }
-      }
-      __syncthreads();
+  auto order = [](u64& x, u64& y, bool up) {
+    if ((x > y) == up) {
+      const u64 t = x;
+      x = y;
+      y = t;
     }
-    // strides inside 32 neighbours: one warp, in registers
-    const int lane = threadIdx.x & 31;
-    for (int base = 32 * (int)(threadIdx.x >> 5); base < p; base += NT) {
-      u64 x = S.list[base + lane];
-      for (int stride = min(size >> 1, 16); stride > 0; stride >>= 1) {
-        const u64 y = __shfl_xor_sync(0xffffffffu, x, stride);
-        const bool up = ((base + lane) & size) == 0, low = (lane & stride) == 0;
-        if ((up == low) ? y < x : y > x) x = y;
+  };
+  auto in_warp = [&](u64& x, int stride, bool up) {
+    const u64 y = __shfl_xor_sync(0xffffffffu, x, stride);
+    if ((up == ((lane & stride) == 0)) ? y < x : y > x) x = y;
+  };
+  for (int size = 64; size <= p; size <<= 1) {
+    int stride = size >> 1;
+    if (size > 64) {
+      if ((__ffs(size) & 1) == 0) {  // an odd number of strides above 32: one alone
+        for (int i = threadIdx.x; i < p / 2; i += NT) {
+          const int a = ((i & ~(stride - 1)) << 1) | (i & (stride - 1));
+          u64 x = S.list[a], y = S.list[a + stride];
+          order(x, y, (a & size) == 0);
+          S.list[a] = x;
+          S.list[a + stride] = y;
+        }
+        __syncthreads();
+        stride >>= 1;
+      }
+      for (; stride > 32; stride >>= 2) {
+        const int half = stride >> 1;
+        for (int i = threadIdx.x; i < p / 4; i += NT) {
+          const int a = ((i & ~(half - 1)) << 2) | (i & (half - 1));
+          const bool up = (a & size) == 0;
+          u64 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = S.list[a + k * half];
+          order(w[0], w[2], up);
+          order(w[1], w[3], up);
+          order(w[0], w[1], up);
+          order(w[2], w[3], up);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) S.list[a + k * half] = w[k];
+        }
+        __syncthreads();
+      }
+    }
+    for (int base = 64 * (int)(threadIdx.x >> 5); base < p; base += 2 * NT) {
+      u64 x = S.list[base + lane], y = S.list[base + 32 + lane];
+      if (size == 64) {
+#pragma unroll
+        for (int z = 2; z <= 32; z <<= 1)
+#pragma unroll
+          for (int t = z >> 1; t > 0; t >>= 1) {
+            in_warp(x, t, (lane & z) == 0);
+            in_warp(y, t, z < 32 && (lane & z) == 0);
+          }
+      }
+      const bool up = (base & size) == 0;
+      order(x, y, up);
+#pragma unroll
+      for (int t = 16; t > 0; t >>= 1) {
+        in_warp(x, t, up);
+        in_warp(y, t, up);
       }
       S.list[base + lane] = x;
+      S.list[base + 32 + lane] = y;
     }
     __syncthreads();
   }
@@ -938,11 +1000,22 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       else pass(No{}, No{});
     }
     hand_over();
-    z.all = block_sum<NT>(z.all, S);
-    if (by_m) z.enough = block_sum<NT>(z.enough, S);
-    z.before_r = block_sum<NT>(z.before_r, S);
-    if (two) z.before_q = block_sum<NT>(z.before_q, S);
-    if (tid == 0) remote(0).sums[rank] = z;
+    // the block's four sums, a warp each
+    u64 v[4] = {z.all, z.enough, z.before_r, z.before_q};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      if (lane == 0) S.reds[k][warp] = v[k];
+    }
+    __syncthreads();
+    if (warp < 4) {
+      u64 t = lane < kWarps ? S.reds[warp][lane] : 0ull;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      Sums& D = remote(0).sums[rank];
+      if (lane == 0) (warp == 0 ? D.all : warp == 1 ? D.enough : warp == 2 ? D.before_r : D.before_q) = t;
+    }
     sync_all();
   };
   if (rank != 0) {
@@ -984,11 +1057,10 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   const double wide = 1.0 + 0x1p-13 - step * step * step / 24.0;
   auto window = [&](double lo, double mid, double hi, int most, int* b0, int* b1) {
     const double total = S.est[kBins - 1];
-    int l = first_bin<NT>(S.est, fmin(lo / wide, total), S), h = first_bin<NT>(S.est, fmin(hi * wide, total), S);
-    int m = first_bin<NT>(S.est, fmin(mid, total), S);
-    l = max(l, 0);
-    h = h < 0 ? kBins - 1 : h;
-    m = max(l, min(m < 0 ? kBins - 1 : m, h));
+    int at[3];
+    first_bins<NT>(S.est, {fmin(lo / wide, total), fmin(mid, total), fmin(hi * wide, total)}, at, S);
+    int l = max(at[0], 0), h = at[2] < 0 ? kBins - 1 : at[2];
+    const int m = max(l, min(at[1] < 0 ? kBins - 1 : at[1], h));
     if (held(l, h) > most) {
       const int side = max(0, most - held(m, m)) / 2;
       const double below = (double)(m > 0 ? S.tcnt[m - 1] : 0u) - side, above = (double)S.tcnt[m] + side + 1.0;
@@ -1016,6 +1088,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       const int most = lane == 0 ? r0 - 1 : lane == 1 ? r1 : lane == 2 ? q0 - 1 : q1;
       auto reached = [&](float v) { return lane < 4 ? bin(v) <= most : R.mass(v) >= p.min_p; };
       uint32_t under = fkey(R.floor) - 1u, upper = fkey(top);  // under: not reached (or no mass); upper: reached
+      if (lane >= (by_m ? 5 : 4)) under = upper - 1u;  // (nothing to find)
       const bool any = lane < 4 ? bin(top) <= most : true;  // (else no logit is)
       while (__any_sync(0xffffffffu, upper - under > 1u)) {
         const uint32_t mid = under + (upper - under) / 2u;
@@ -1057,8 +1130,10 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       run[k] = t;
     }
     const u64 e = block_scan<NT>(t, S);
-    inside = block_sum<NT>(inside, S);
-    n_r = (int)block_sum<NT>((u64)here, S);
+    if (q0 <= q1) {
+      inside = block_sum<NT>(inside, S);
+      n_r = (int)block_sum<NT>((u64)here, S);
+    }
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
       const int i = kPerList * tid + k;
