@@ -378,11 +378,17 @@ typedef struct nls_g4_weights {
  *  x  nb rows of cols activations of type xtype, ldx >= cols values apart
  *  y  nb rows of w->rows values of type ytype, ldy >= w->rows apart; what lies
  *     behind a row's w->rows values is left as it was
- * Products of a 4-bit value and an activation are exact (fp32 activations are
- * taken as three bfloat16 parts); they are summed in fp32 per group, the
- * groups' terms in fp32, and rounded once to ytype. fp32 and bfloat16
+ * Weights are not rounded on the way. Up to 12 batch rows (4 with groups of
+ * 32): activations enter as fixed-point numbers of 31 bits against the largest
+ * magnitude of the row's 128 columns around them (each is off by 2^-31 of that
+ * magnitude at most), and a group's products are summed exactly, in integers.
+ * More rows: the products are exact (fp32 activations are taken as three
+ * bfloat16 parts) and are summed in fp32 per group; fp32 and bfloat16
  * activations are shifted by 2^-12 on the way, so that sums before the scales
- * cannot overflow; what they lose lies below 2^-110. A batch row that holds an
+ * cannot overflow, and what they lose lies below 2^-110. Either way the
+ * groups' terms are summed in fp32 and rounded once to ytype; a row's bits
+ * depend on nb through the way taken. Scales and minimums are below 2^80 in
+ * magnitude (larger ones may overflow inside). A batch row that holds an
  * infinity or a NaN gets non-finite logits; the other rows are unaffected.
  * The same call gives the same bits every time. A pipeline wait that runs out
  * (nls_set_wait_limit) gives NLS_ERR_TIMEOUT and leaves y undefined.

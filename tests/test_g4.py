@@ -2,10 +2,13 @@
 64 bits.
 
 Tolerance. With q' = q - 8 the kernel computes s * sum(q' x) + m' * sum(x),
-m' = m + 8 s, per group: products of a 4-bit and a 16-bit (or a third of an
-fp32) value are exact in fp32, and every other operation rounds to fp32 or, in
-the tensor core's accumulator, cuts off, so is off by at most 2^-23 relative
-to the sum of magnitudes so far. A logit is a sum of at most `group` terms,
+m' = m + 8 s, per group. More than 12 batch rows (4 with groups of 32):
+products of a 4-bit and a 16-bit (or a third of an fp32) value are exact in
+fp32, and every other operation rounds to fp32 or, in the tensor core's
+accumulator, cuts off, so is off by at most 2^-23 relative to the sum of
+magnitudes so far. Fewer rows: the inner sums are exact but for each x, which is
+off by 2^-31 of the largest of its 128 columns; where activations are of one
+size that is far below 2^-23 of the sum (a test of its own has one that is not). A logit is a sum of at most `group` terms,
 then of the groups' terms, with fewer than 8 further roundings (m', its sum,
 the scalings, the parts of a split tile), so it is within
 (group + 3 * groups + 8) * 2^-23 * A of the exact value, A the same sum of
@@ -199,6 +202,31 @@ def test_fp32_activations_keep_their_low_bits(pkg, eng):
     top = torch.full((256,), 3.0e37)                       # rounds up, not to infinity
     top[::2] = -3.0e37
     check(w, top[None].cuda(), eng.g4_matmul(w, top[None].cuda()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("nb", [1, 4, 12, 16])
+def test_an_activation_much_larger_than_its_neighbours(pkg, eng, nb, mins):
+    """Within the tolerance, and with few batch rows 2^-31 of the row's largest
+    activation of 128 columns, times the magnitude of each weight of theirs."""
+    import torch
+    rows, cols, group = 700, 640, 64
+    w = make(pkg, rows, cols, group, "f16", mins, seed=9)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn((nb, cols), generator=g)
+    x[:, 5] = 3e6
+    x[:, 300] = -2e8
+    x = x.cuda()
+    W, A = parts(w)
+    xd = x.double()
+    tol = (group + 3 * (cols // group) + 8) * 2.0 ** -23 * (xd.abs() @ A.t())
+    if nb <= 12:
+        top = xd.abs().reshape(nb, -1, 128).amax(2, keepdim=True).expand(nb, cols // 128, 128).reshape(nb, cols)
+        tol = tol + 2.0 ** -31 * (top @ A.t())
+    err = (eng.g4_matmul(w, x).double() - xd @ W.t()).abs()
+    tol = tol + (xd @ W.t()).abs() * 2.0 ** -24
+    assert bool((err <= tol).all()), float((err / tol).max())
 
 
 @pytest.mark.gpu
