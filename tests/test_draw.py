@@ -389,3 +389,74 @@ def test_a_generation_loop(pkg, eng):
         want = [row_reference(x[r], P[r], float(us[t, r]))[0] for r in range(B)]
         assert seen[t].tolist() == want
         tok = seen[t]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nb", [2, 20])
+def test_a_captured_step(pkg, eng, nb):
+    """Projection and draw captured together, replayed on new inputs, also after
+    a larger call on the handle."""
+    import torch
+    g = torch.Generator().manual_seed(nb)
+    V, D = 9001, 512
+    w = pkg.g4_quantize(torch.randn((V, D), generator=g).cuda() * 0.1, group=64, symmetric=False, dtype=torch.float16)
+    rng = np.random.default_rng(nb)
+    P = settings(pkg, rng, nb, V)
+    Pd = torch.from_numpy(P.view(np.uint8).copy()).cuda()
+    x, u = torch.randn((nb, D), generator=g).half().cuda(), torch.from_numpy(rng.random(nb)).cuda()
+    ids = torch.zeros(nb, dtype=torch.int64, device="cuda")
+    probs = torch.zeros(nb, device="cuda")
+    fresh = pkg.Engine(0, max_rows=256, max_vocab=1 << 14)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        fresh.g4_lm_head_draw(w, x, Pd, u, logits_dtype=torch.float32, out_ids=ids, out_probs=probs)
+        with torch.cuda.graph(graph):
+            fresh.g4_lm_head_draw(w, x, Pd, u, logits_dtype=torch.float32, out_ids=ids, out_probs=probs, check=False)
+        many = torch.randn((250, D), generator=g).half().cuda()
+        fresh.g4_lm_head_draw(w, many, pkg.draw_params(250, top_k=5), np.full(250, 0.5), logits_dtype=torch.float32)
+        for _ in range(3):
+            x.copy_(torch.randn((nb, D), generator=g).half())
+            u.copy_(torch.from_numpy(rng.random(nb)))
+            graph.replay()
+            torch.cuda.synchronize()
+            logits = eng.g4_matmul(w, x, out_dtype=torch.float32)
+            check(ids, probs, logits, P, u.cpu().numpy())
+    finally:
+        del graph
+        fresh.close()
+
+
+@pytest.mark.gpu
+def test_two_handles_at_once(pkg, eng):
+    """Calls on two handles and two streams, side by side."""
+    import torch
+    g = torch.Generator().manual_seed(3)
+    V, D, steps = 30011, 1024, 20
+    w = pkg.g4_quantize(torch.randn((V, D), generator=g).cuda() * 0.1, group=128, dtype=torch.float16)
+    sizes = (3, 24)
+    rng = np.random.default_rng(3)
+    P = [settings(pkg, rng, n, V) for n in sizes]
+    Pd = [torch.from_numpy(p.view(np.uint8).copy()).cuda() for p in P]
+    x = [torch.randn((steps, n, D), generator=g).half().cuda() for n in sizes]
+    u = [torch.from_numpy(rng.random((steps, n))).cuda() for n in sizes]
+    want = [[eng.g4_lm_head_draw(w, x[i][t], Pd[i], u[i][t], logits_dtype=torch.bfloat16)[:2] for t in range(steps)]
+            for i in range(2)]
+    handles = [pkg.Engine(0, max_rows=32, max_vocab=1 << 15) for _ in sizes]
+    streams = [torch.cuda.Stream() for _ in sizes]
+    try:
+        for i in range(2):  # (the workspaces)
+            handles[i].g4_lm_head_draw(w, x[i][0], Pd[i], u[i][0], logits_dtype=torch.bfloat16)
+        torch.cuda.synchronize()
+        got = [[], []]
+        for t in range(steps):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(handles[i].g4_lm_head_draw(w, x[i][t], Pd[i], u[i][t], logits_dtype=torch.bfloat16,
+                                                             check=False)[:2])
+        torch.cuda.synchronize()
+        for i in range(2):
+            for t in range(steps):
+                assert torch.equal(got[i][t][0], want[i][t][0]) and torch.equal(got[i][t][1], want[i][t][1])
+    finally:
+        for h in handles:
+            h.close()
