@@ -219,13 +219,28 @@ __device__ void first_bins(const double* run, const double (&target)[3], int (&b
   for (int k = 0; k < 3; ++k) bin[k] = S.picks[k];
 }
 
-// S.list[0 .. n) ascending (n <= kList): bitonic. A warp keeps 64 neighbours in
+// S.list[0 .. n) ascending (n <= kList). Short lists by counting: four lanes find
+// a token's place (all differ). Longer ones bitonic: a warp keeps 64 neighbours in
 // registers for the strides below 64; larger strides go through shared memory,
 // two at a time. (Few barriers: with one stride each, 555 tokens took 17000
 // cycles.)
 template <int NT>
 __device__ void sort_list(int n, Shared& S) {
   const int lane = threadIdx.x & 31;
+  if (n <= NT / 4) {
+    const int i = threadIdx.x >> 2;
+    __syncthreads();
+    const u64 x = S.list[min(i, n)];
+    int place = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < n; j += 4) place += S.list[j] < x ? 1 : 0;
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    place += __shfl_xor_sync(0xffffffffu, place, 2);
+    __syncthreads();
+    if (i < n && (threadIdx.x & 3) == 0) S.list[place] = x;
+    __syncthreads();
+    return;
+  }
   int p = 64;
   while (p < n) p <<= 1;
   for (int i = n + (int)threadIdx.x; i < p; i += NT) S.list[i] = ~0ull;
@@ -806,14 +821,16 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   };
 
   int n = 0;           // tokens in the list
-  u64 run[kPerList];   // the running masses of this thread's neighbours in it
+  int per = 1;         // neighbours in it per thread (kPerList where they are more than threads)
+  u64 run[kPerList];   // their running masses
+  auto place = [&](int k) { return k < per ? per * tid + k : INT_MAX; };
   // the first of them whose running mass reaches target: its place in the
   // list (-1: none), and that mass in S.value
   auto reach = [&](double target) -> int {
     int at = INT_MAX;
 #pragma unroll
     for (int k = kPerList - 1; k >= 0; --k)
-      if (kPerList * tid + k < n && (double)run[k] >= target) at = kPerList * tid + k;
+      if (place(k) < n && (double)run[k] >= target) at = place(k);
     at = __reduce_min_sync(0xffffffffu, at);
     __syncthreads();
     if (tid == 0) S.pick = INT_MAX;
@@ -824,7 +841,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     if (i == INT_MAX) return -1;
 #pragma unroll
     for (int k = 0; k < kPerList; ++k)
-      if (i == kPerList * tid + k) S.value = run[k];
+      if (i == place(k)) S.value = run[k];
     __syncthreads();
     return i;
   };
@@ -874,12 +891,12 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       }
       sort_list<NT>(n, S);
       if (by_k) n = min(n, (int)p.top_k);  // tokens kept by top-k
+      per = n <= NT ? 1 : kPerList;
       u64 t = 0;
       unsigned enough = 0;  // which of them have at least min_p
 #pragma unroll
       for (int k = 0; k < kPerList; ++k) {
-        const int i = kPerList * tid + k;
-        const float v = i < n ? Row::value(S.list[i]) : -INFINITY;
+        const float v = place(k) < n ? Row::value(S.list[place(k)]) : -INFINITY;
         const double m = R.has_mass(v) ? R.mass(v) : 0.0;
         if (!by_m || !(m < p.min_p)) enough |= 1u << k;
         t += Row::units(m);
@@ -896,7 +913,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 #pragma unroll
       for (int k = 0; k < kPerList; ++k) {
         run[k] += e;
-        if (kPerList * tid + k < n && (!by_p || (double)prev < tp) && (enough & (1u << k))) kept = run[k];
+        if (place(k) < n && (!by_p || (double)prev < tp) && (enough & (1u << k))) kept = run[k];
         prev = run[k];
       }
       __syncthreads();
@@ -1118,13 +1135,13 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
     if (n > kList) return false;
     sort_list<NT>(n, S);
+    per = n <= NT ? 1 : kPerList;
     u64 t = 0, inside = 0;  // inside: the tokens of r0 .. r1, n_r of them
     int here = 0;
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
-      const int i = kPerList * tid + k;
-      if (i < n) {
-        const float v = Row::value(S.list[i]);
+      if (place(k) < n) {
+        const float v = Row::value(S.list[place(k)]);
         const u64 w = R.units_of(v);
         t += w;
         if (v >= c.rb) {
@@ -1141,8 +1158,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
 #pragma unroll
     for (int k = 0; k < kPerList; ++k) {
-      const int i = kPerList * tid + k;
-      const bool first = i >= n || Row::value(S.list[i]) >= c.rb;
+      const bool first = place(k) >= n || Row::value(S.list[place(k)]) >= c.rb;
       run[k] += e + (first ? z.before_r : z.before_q - inside);
     }
     return true;
@@ -1162,7 +1178,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kPerList; ++k)
-          if (i == kPerList * tid + k) S.value = run[k];
+          if (i == place(k)) S.value = run[k];
         __syncthreads();
         total = S.value;
         total_est = (double)total / kUnit;
