@@ -34,8 +34,8 @@
 // What bounds it: reading the logits for the first way; for the second the
 // instructions of the masses (about 40 per logit, 11 of them fp64, in the exact
 // pass); for a few rows the chain of barriers of one row. Measured: 256 x 128256
-// fp32, highest logit 29 us (4.5 TB/s), top-k 50 43 us, nucleus 160 us, settings
-// of every kind 112 us; 2048 x 151936 bfloat16 top-k 50 262 us (2.4 TB/s); 64 x
+// fp32, highest logit 29 us (4.5 TB/s), top-k 50 43 us, nucleus 157 us, settings
+// of every kind 110 us; 2048 x 151936 bfloat16 top-k 50 252 us (2.5 TB/s); 64 x
 // 151936 bfloat16 nucleus 72 us; one row of 128256: top-k with top-p and min-p
 // 19 us, nucleus 36 us.
 #include <cooperative_groups.h>

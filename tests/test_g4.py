@@ -179,6 +179,22 @@ def test_every_batch_size(pkg, eng, nb, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nb", [200, 300, 333])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+def test_many_batch_rows(pkg, eng, nb, group, xt):
+    """More passes than the workspace is planned for one by one."""
+    import torch
+    w = make(pkg, 515, 288, group, "f16", True, seed=nb)
+    x = torch.randn((nb, 288), generator=torch.Generator().manual_seed(nb)).to(_dt(xt)).cuda()
+    fresh = pkg.Engine(0, max_rows=1, max_vocab=1024)
+    try:
+        check(w, x, fresh.g4_matmul(w, x, out_dtype=torch.float32))
+    finally:
+        fresh.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("st", DTYPES)
 @pytest.mark.parametrize("xt", DTYPES)
 @pytest.mark.parametrize("yt", DTYPES)
