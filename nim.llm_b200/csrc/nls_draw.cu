@@ -1275,7 +1275,8 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
     if ((int64_t)C * a.rows > sm_count && nvec > 128) {
       // 1024 threads to an SM: four rows, or two where there are not that many
       // (256 x 128256 fp32 with 512 and with 1024 threads a row: top-k 43 and 55
-      // us, nucleus 160 and 169, settings of every kind 111 and 98)
+      // us, nucleus 160 and 169, settings of every kind 111 and 98; 2048 x 151936
+      // bfloat16 top-k with 256 and with 512 threads: 253 and 270 us)
       const bool many = a.rows > 3 * sm_count;
       auto stream = [&](auto kernel, int threads, std::atomic<int>* set) {
         cudaError_t f = ensure_smem_attr(reinterpret_cast<const void*>(kernel), (int)smem_bytes(0), set);
