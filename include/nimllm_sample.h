@@ -427,6 +427,8 @@ typedef struct nls_draw_params {
  *  params    [rows]
  *  uniforms  [rows] in [0, 1); NULL only if every row has temperature <= 0
  *  out_ids   [rows]; out_probs [rows] or NULL (1 for temperature <= 0)
+ * Device arrays are aligned to their type (params and uniforms to 8 bytes):
+ * NLS_ERR_INVALID_ARG otherwise.
  * A row that holds a NaN, whose maximum is +inf or that is -inf throughout
  * gets id -1, probability 0 and NLS_ERR_NAN_LOGITS; a NaN temperature or a
  * uniform outside [0, 1) gets id -1 and NLS_ERR_INVALID_ARG. -inf logits are

@@ -756,6 +756,17 @@ nls_status draw_impl(nls_handle* h, const void* logits, int32_t ltype, int64_t l
 
 constexpr uint32_t kDevFlags = NLS_DEVICE_INPUTS | NLS_DEVICE_OUTPUTS;
 
+// The arrays of a draw that its kernel reads and writes in place: there, each
+// aligned to its type (host arrays are copied by bytes).
+bool draw_arrays_ok(const nls_draw_params* params, const double* uniforms, const int64_t* out_ids,
+                    const float* out_probs, uint32_t flags) {
+  if (!params || !out_ids) return false;
+  if ((flags & NLS_DEVICE_INPUTS) &&
+      !(aligned_to(params, alignof(nls_draw_params)) && aligned_to(uniforms, alignof(double))))
+    return false;
+  return !(flags & NLS_DEVICE_OUTPUTS) || (aligned_to(out_ids, alignof(int64_t)) && aligned_to(out_probs, alignof(float)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -796,7 +807,8 @@ nls_status nls_draw_batch(nls_handle* h, const void* logits, int32_t ltype, int6
   if (!h || (flags & ~kDevFlags)) return NLS_ERR_INVALID_ARG;
   if (rows < 0 || vocab < 1 || ld < vocab || !nls::dt_ok(ltype)) return NLS_ERR_INVALID_ARG;
   if (rows == 0) return NLS_OK;
-  if (!logits || !aligned_to(logits, nls::dt_size(ltype)) || !params || !out_ids) return NLS_ERR_INVALID_ARG;
+  if (!logits || !aligned_to(logits, nls::dt_size(ltype))) return NLS_ERR_INVALID_ARG;
+  if (!draw_arrays_ok(params, uniforms, out_ids, out_probs, flags)) return NLS_ERR_INVALID_ARG;
   if (rows > h->max_rows || vocab > h->max_vocab) return NLS_ERR_CAPACITY;
   DeviceGuard g(h->device);
   cudaStream_t st = (cudaStream_t)stream;
@@ -812,7 +824,8 @@ nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, const voi
   if (!h || (flags & ~kDevFlags) || rows < 0) return NLS_ERR_INVALID_ARG;
   if (!g4_weights_ok(w) || !nls::dt_ok(xtype) || !nls::dt_ok(ltype) || ldx < w->cols) return NLS_ERR_INVALID_ARG;
   if (rows == 0) return NLS_OK;
-  if (!x || !aligned_to(x, nls::dt_size(xtype)) || !params || !out_ids) return NLS_ERR_INVALID_ARG;
+  if (!x || !aligned_to(x, nls::dt_size(xtype))) return NLS_ERR_INVALID_ARG;
+  if (!draw_arrays_ok(params, uniforms, out_ids, out_probs, flags)) return NLS_ERR_INVALID_ARG;
   if (rows > h->max_rows || w->rows > h->max_vocab) return NLS_ERR_CAPACITY;
   DeviceGuard g(h->device);
   cudaStream_t st = (cudaStream_t)stream;

@@ -460,3 +460,28 @@ def test_two_handles_at_once(pkg, eng):
     finally:
         for h in handles:
             h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["params", "uniforms", "out_ids", "out_probs"])
+def test_misaligned_device_arrays_are_refused(pkg, eng, which):
+    """Before anything is launched; host arrays may lie anywhere."""
+    import ctypes
+    import torch
+    lib = pkg.load()
+    w = pkg.g4_quantize(torch.ones((64, 128), device="cuda"), group=128)
+    x = torch.zeros((2, 128), device="cuda")
+    at = {n: torch.zeros(128, dtype=torch.uint8, device="cuda") for n in ("params", "uniforms", "out_ids", "out_probs")}
+    ptr = [t.data_ptr() + (2 if n == which == "out_probs" else 4 if n == which else 0) for n, t in at.items()]
+    assert lib.nls_draw_batch(eng._h, x.data_ptr(), 0, 64, 2, 64, *ptr, 3, None) == 1
+    assert lib.nls_g4_lm_head_draw(eng._h, ctypes.byref(w.struct), x.data_ptr(), 0, 128, 2, 0, *ptr, 3, None) == 1
+    if which == "params":
+        with pytest.raises(pkg.NlsError) as e:
+            eng.draw_batch(x, at["params"][4:68], torch.zeros(2, dtype=torch.float64, device="cuda"))
+        assert e.value.status == pkg._abi.NLS_ERR_INVALID_ARG
+    host = np.zeros(256, np.uint8)
+    host[1:65] = pkg.draw_params(2).view(np.uint8)
+    base = host.ctypes.data + 1
+    logits = np.zeros((2, 64), np.float32)
+    assert lib.nls_draw_batch(eng._h, logits.ctypes.data, 0, 64, 2, 64, base, base + 64, base + 80, base + 96, 0, None) == 0
+    assert host[81:97].view(np.int64).tolist() == [0, 0]
