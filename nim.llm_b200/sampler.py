@@ -357,8 +357,10 @@ class Engine:
         return torch.cuda.current_stream(self.device).cuda_stream
 
     def _finish(self, st: int, what: str, cuda: bool, stream, check: bool) -> int:
-        """Raise on a call's error. Arguments and launches are always checked;
-        the kernels' status of a device call only with `check` (it waits)."""
+        """Raise on a call's error and return its status. A device call's
+        arguments and launches are always checked, its kernels' status only
+        with `check` (it waits); a host call has waited, and with check=False
+        its status is the caller's to look at."""
         if st != 0 and (check or cuda):
             self._check(st, what)
         if cuda and check:
@@ -385,7 +387,8 @@ class Engine:
         """x . W^T for 4-bit weights (G4Weights): [nb, rows] of `out_dtype` (x's
         by default). x [nb, cols] or [cols], a CUDA tensor (stream-ordered on
         `stream`, torch's current one by default; check=False does not wait for
-        the kernels) or a CPU tensor (returns a CPU tensor)."""
+        the kernels) or a CPU tensor (returns a CPU tensor; a failed call always
+        raises)."""
         import torch
         cuda = x.is_cuda
         weights = self._g4_weights(w)
@@ -407,7 +410,7 @@ class Engine:
             st = self._lib.nls_g4_matmul(
                 self._h, weights, xp, _g4.dt_code(x.dtype), ldx, nb, yp, _g4.dt_code(y.dtype), ldy,
                 _abi.NLS_DEVICE_INPUTS | _abi.NLS_DEVICE_OUTPUTS if cuda else 0, sp)
-            self._finish(st, "nls_g4_matmul", cuda, sp, check)
+            self._finish(st, "nls_g4_matmul", cuda, sp, check or not cuda)
         return out if out is not None else (y[0] if x.dim() == 1 else y)
 
     def _draw_inputs(self, B, params, uniforms, out_ids, out_probs, cuda):
@@ -454,7 +457,8 @@ class Engine:
         CUDA tensor: params (draw_params records, or a device tensor of 32
         bytes per row) and float64 uniforms; results are CUDA tensors, the call
         is stream-ordered (check=False does not wait). CPU tensor or numpy
-        array: numpy params, uniforms and results."""
+        array: numpy params, uniforms and results (check=False returns a failed
+        call's status instead of raising)."""
         import torch
         if not _is_torch(logits):
             logits = torch.from_numpy(np.ascontiguousarray(logits))

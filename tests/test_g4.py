@@ -130,6 +130,38 @@ def test_struct_layout_matches_c(pkg, tmp_path):
     assert vals[2 + len(names):] == [pkg.DRAW_PARAMS_DTYPE.fields[n][1] for n in dn]
 
 
+def test_a_failed_host_call_raises_with_check_off(pkg):
+    """check=False does not wait for a device call's kernels; a host call has
+    waited, and its result is not handed out when it has failed."""
+    import types
+    import torch
+    w = types.SimpleNamespace(device=torch.device("cuda", 0), struct=pkg._abi.G4WeightsStruct(), rows=16, cols=64)
+
+    class Lib:
+        status = 0
+
+        def nls_g4_matmul(self, *args):
+            return self.status
+
+        def nls_last_error(self, h):
+            return b""
+
+        def nls_destroy(self, h):
+            pass
+
+    eng = pkg.Engine.__new__(pkg.Engine)
+    eng._lib, eng._h, eng.device, eng._torch_device = Lib(), None, 0, None
+    x = torch.zeros((2, 64))
+    for check in (True, False):
+        Lib.status = 0
+        assert eng.g4_matmul(w, x, check=check).shape == (2, 16)
+        for status in (pkg._abi.NLS_ERR_TIMEOUT, pkg._abi.NLS_ERR_CUDA, pkg._abi.NLS_ERR_INVALID_ARG):
+            Lib.status = status
+            with pytest.raises(pkg.NlsError) as e:
+                eng.g4_matmul(w, x, check=check)
+            assert e.value.status == status
+
+
 # ---- GPU ------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
