@@ -756,6 +756,14 @@ nls_status draw_impl(nls_handle* h, const void* logits, int32_t ltype, int64_t l
 
 constexpr uint32_t kDevFlags = NLS_DEVICE_INPUTS | NLS_DEVICE_OUTPUTS;
 
+// A call without rows launches nothing, but it is the stream's last call: what
+// nls_stream_status reads afterwards is its success, not an earlier call's error.
+nls_status empty_call(nls_handle* h, cudaStream_t st) {
+  DeviceGuard g(h->device);
+  NLS_CUDA(h, cudaMemsetAsync(h->d_work, 0, sizeof(int), st));
+  return NLS_OK;
+}
+
 // The arrays of a draw that its kernel reads and writes in place: there, each
 // aligned to its type (host arrays are copied by bytes).
 bool draw_arrays_ok(const nls_draw_params* params, const double* uniforms, const int64_t* out_ids,
@@ -777,7 +785,7 @@ nls_status nls_g4_matmul(nls_handle* h, const nls_g4_weights* w, const void* x, 
   if (!h || (flags & ~kDevFlags) || nb < 0) return NLS_ERR_INVALID_ARG;
   if (!g4_weights_ok(w) || !nls::dt_ok(xtype) || !nls::dt_ok(ytype)) return NLS_ERR_INVALID_ARG;
   if (ldx < w->cols || ldy < w->rows) return NLS_ERR_INVALID_ARG;
-  if (nb == 0) return NLS_OK;
+  if (nb == 0) return empty_call(h, (cudaStream_t)stream);
   if (!x || !y || !aligned_to(x, nls::dt_size(xtype)) || !aligned_to(y, nls::dt_size(ytype)))
     return NLS_ERR_INVALID_ARG;
   DeviceGuard g(h->device);
@@ -806,7 +814,7 @@ nls_status nls_draw_batch(nls_handle* h, const void* logits, int32_t ltype, int6
                           int64_t* out_ids, float* out_probs, uint32_t flags, void* stream) {
   if (!h || (flags & ~kDevFlags)) return NLS_ERR_INVALID_ARG;
   if (rows < 0 || vocab < 1 || ld < vocab || !nls::dt_ok(ltype)) return NLS_ERR_INVALID_ARG;
-  if (rows == 0) return NLS_OK;
+  if (rows == 0) return empty_call(h, (cudaStream_t)stream);
   if (!logits || !aligned_to(logits, nls::dt_size(ltype))) return NLS_ERR_INVALID_ARG;
   if (!draw_arrays_ok(params, uniforms, out_ids, out_probs, flags)) return NLS_ERR_INVALID_ARG;
   if (rows > h->max_rows || vocab > h->max_vocab) return NLS_ERR_CAPACITY;
@@ -823,7 +831,7 @@ nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, const voi
                                uint32_t flags, void* stream) {
   if (!h || (flags & ~kDevFlags) || rows < 0) return NLS_ERR_INVALID_ARG;
   if (!g4_weights_ok(w) || !nls::dt_ok(xtype) || !nls::dt_ok(ltype) || ldx < w->cols) return NLS_ERR_INVALID_ARG;
-  if (rows == 0) return NLS_OK;
+  if (rows == 0) return empty_call(h, (cudaStream_t)stream);
   if (!x || !aligned_to(x, nls::dt_size(xtype))) return NLS_ERR_INVALID_ARG;
   if (!draw_arrays_ok(params, uniforms, out_ids, out_probs, flags)) return NLS_ERR_INVALID_ARG;
   if (rows > h->max_rows || w->rows > h->max_vocab) return NLS_ERR_CAPACITY;

@@ -485,3 +485,21 @@ def test_misaligned_device_arrays_are_refused(pkg, eng, which):
     logits = np.zeros((2, 64), np.float32)
     assert lib.nls_draw_batch(eng._h, logits.ctypes.data, 0, 64, 2, 64, base, base + 64, base + 80, base + 96, 0, None) == 0
     assert host[81:97].view(np.int64).tolist() == [0, 0]
+
+
+@pytest.mark.gpu
+def test_an_empty_batch_has_no_error_of_an_earlier_call(pkg, eng):
+    import torch
+    w = pkg.g4_quantize(torch.ones((64, 128), device="cuda"), group=128)
+    x = torch.zeros((2, 128), device="cuda")
+    nan = torch.full((1, 64), float("nan"), device="cuda")
+    P, u = pkg.draw_params(1), np.zeros(1)
+    none, no_u = pkg.draw_params(0), np.zeros(0)
+    for empty in (lambda: eng.draw_batch(nan[:0], none, no_u)[0].numel(),
+                  lambda: eng.g4_matmul(w, x[:0]).numel(),
+                  lambda: eng.g4_lm_head_draw(w, x[:0], none, no_u)[0].numel()):
+        ids, _, _ = eng.draw_batch(nan, P, u, check=False)
+        assert empty() == 0
+        assert ids.tolist() == [-1]
+        with pytest.raises(pkg.NlsError):                  # (the earlier call's error is its own)
+            eng.draw_batch(nan, P, u)
