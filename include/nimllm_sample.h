@@ -238,12 +238,13 @@ NLS_API nls_status nls_sample_batch_vocab_sharded(
 
 /* Limit, in nanoseconds, of the bounded waits in which the streaming kernel
  * (greedy and top-k <= 256 rows) waits for its bulk copies of logits, and
- * in which the tensor-core path of nls_lm_head waits between its pipeline
- * stages (default 200 ms; later calls on this handle use it). A wait that
- * runs out fails its row (id -1) or the projection with NLS_ERR_TIMEOUT,
- * after the kernel has waited, with the default limit, for the copies (and
- * MMAs) it has in flight. A limit of 0 is a
- * deadline already past: every such wait gives up at once, which drives that
+ * in which the tensor-core path of nls_lm_head and every nls_g4_matmul (and
+ * the same projections in nls_lm_head_sample and nls_g4_lm_head_draw) wait
+ * between their pipeline stages (default 200 ms; later calls on this handle
+ * use it). A wait that runs out fails its row (id -1) or the projection with
+ * NLS_ERR_TIMEOUT, after the kernel has waited, with the default limit, for
+ * the copies (and MMAs) it has in flight. A limit of 0 is a deadline already
+ * past: every such wait gives up at once, which drives that
  * failure path on purpose (tests of the timeout handling). No counterpart in
  * the reference (its sampler runs on the host and waits for nothing). */
 NLS_API nls_status nls_set_wait_limit(nls_handle* h, uint64_t ns);
@@ -451,8 +452,9 @@ NLS_API nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, c
 
 /* Per-kernel timing of later calls on this handle (tracing; no counterpart
  * in the reference, which only times whole generations with epochTime,
- * chat.nim:191,246-247). With `on` set, every sampling call records CUDA
- * events around each of its kernels on the call's stream. */
+ * chat.nim:191,246-247). With `on` set, every sampling call (draws included)
+ * records CUDA events around each of its kernels on the call's stream; the
+ * projections are not timed, in calls that do both neither. */
 NLS_API nls_status nls_set_profiling(nls_handle* h, int32_t on);
 
 /* Device times in milliseconds of the last profiled call, each measured from
@@ -461,7 +463,8 @@ NLS_API nls_status nls_set_profiling(nls_handle* h, int32_t on);
  * full-sort kernel (the other rows; above 8 rows it runs concurrently with the
  * streaming kernel, else after it), out_ms[2] to the end of the call's last
  * kernel (above 8 rows, a second full-sort
- * launch over rows the streaming kernel handed back). Waits for those events.
+ * launch over rows the streaming kernel handed back). A draw is one kernel:
+ * all three are its end. Waits for those events.
  * `n` is the capacity of out_ms (up to 3 values are written). */
 NLS_API nls_status nls_last_kernel_ms(nls_handle* h, float* out_ms, int32_t n);
 

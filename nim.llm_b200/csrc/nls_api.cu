@@ -63,11 +63,11 @@ struct nls_handle {
   cudaStream_t side = nullptr;
   cudaEvent_t fork = nullptr, join = nullptr;
   // profiling: [0] start, [1] streaming kernel done, [2] full-sort kernel
-  // done, [3] fallback launch done
+  // done, [3] fallback launch done (a draw: [1] to [3] its kernel done)
   int profiling = 0;
   int profiled = 0;
   // limit of the streaming kernel's bulk-copy waits and of the tensor-core
-  // output projection's pipeline waits (nls_set_wait_limit)
+  // projections' pipeline waits (nls_set_wait_limit)
   unsigned long long wait_ns = 200ull * 1000ull * 1000ull;
   cudaEvent_t ev[4] = {nullptr, nullptr, nullptr, nullptr};
   // vocab-sharded calls: packed shard, received shards, gathered ids/probs
@@ -744,7 +744,12 @@ nls_status draw_impl(nls_handle* h, const void* logits, int32_t ltype, int64_t l
   }
   a.out_ids = dev_out ? out_ids : h->d_out_ids;
   a.out_probs = dev_out ? out_probs : (out_probs ? h->d_out_probs : nullptr);
+  // (one kernel: the three times are its end)
+  const bool prof = h->profiling != 0;
+  if (prof) NLS_CUDA(h, cudaEventRecord(h->ev[0], st));
   NLS_CUDA(h, nls::launch_draw(a, h->sm_count, st));
+  for (int i = 1; prof && i < 4; ++i) NLS_CUDA(h, cudaEventRecord(h->ev[i], st));
+  h->profiled = prof ? 1 : 0;
   if (dev_out) return NLS_OK;
   NLS_CUDA(h, cudaMemcpyAsync(h->h_status, h->d_work, sizeof(int), cudaMemcpyDeviceToHost, st));
   NLS_CUDA(h, cudaMemcpyAsync(out_ids, h->d_out_ids, sizeof(int64_t) * rows, cudaMemcpyDeviceToHost, st));

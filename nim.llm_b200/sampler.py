@@ -201,8 +201,9 @@ class Engine:
         return out_ids, out_probs
 
     def set_wait_limit(self, ns: int) -> None:
-        """Limit of the streaming kernel's bulk-copy waits, in ns (default
-        200 ms); 0 makes every such wait give up (nls_set_wait_limit)."""
+        """Limit of the streaming kernel's bulk-copy waits and of the tensor-core
+        projections' pipeline waits, in ns (default 200 ms); 0 makes every such
+        wait give up (nls_set_wait_limit)."""
         self._check(self._lib.nls_set_wait_limit(self._h, int(ns)), "nls_set_wait_limit")
 
     def set_profiling(self, on: bool = True) -> None:
@@ -211,7 +212,7 @@ class Engine:
     def last_kernel_ms(self) -> tuple[float, float, float]:
         """Device ms of the last profiled call, each from the call's start: to
         the end of the streaming kernel, of the (concurrent) full-sort kernel,
-        and of the call's last kernel."""
+        and of the call's last kernel (a draw is one kernel: three times its end)."""
         out = (ctypes.c_float * 3)()
         self._check(self._lib.nls_last_kernel_ms(self._h, out, 3), "nls_last_kernel_ms")
         return float(out[0]), float(out[1]), float(out[2])

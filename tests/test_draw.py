@@ -503,3 +503,37 @@ def test_an_empty_batch_has_no_error_of_an_earlier_call(pkg, eng):
         assert ids.tolist() == [-1]
         with pytest.raises(pkg.NlsError):                  # (the earlier call's error is its own)
             eng.draw_batch(nan, P, u)
+
+
+@pytest.mark.gpu
+def test_profiled_times_are_the_last_draws(pkg):
+    """A draw is a sampling call: with profiling on its times replace those of
+    the call before, and with profiling off there are none."""
+    import torch
+    e = pkg.Engine(0, max_rows=512, max_vocab=1 << 17)
+    try:
+        w = pkg.g4_quantize(torch.ones((64, 128), device="cuda"), group=128)
+        big = torch.randn((512, 100000), device="cuda")
+        P, u = pkg.draw_params(512, top_p=0.9), np.full(512, 0.5)
+        e.draw_batch(big, P, u)
+        with pytest.raises(pkg.NlsError):
+            e.last_kernel_ms()
+        e.set_profiling(True)
+        for _ in range(2):
+            e.draw_batch(big, P, u)
+            many = e.last_kernel_ms()
+            # (three events, recorded one after the other behind the one kernel;
+            # 205 MB cannot be read in less)
+            assert 0.02 < many[0] <= many[1] <= many[2]
+            e.draw_batch(big[:1, :64], P[:1], u[:1])
+            one = e.last_kernel_ms()
+            assert 0 < one[2] < many[2]
+            e.draw_batch(big, P, u)
+            e.g4_lm_head_draw(w, torch.zeros((1, 128), device="cuda"), P[:1], u[:1])
+            assert 0 < e.last_kernel_ms()[2] < many[2]
+        e.set_profiling(False)
+        e.draw_batch(big, P, u)
+        with pytest.raises(pkg.NlsError):
+            e.last_kernel_ms()
+    finally:
+        e.close()
