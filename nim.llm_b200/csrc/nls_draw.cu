@@ -1240,7 +1240,8 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
   }
   (void)command(Command{kExit});
-  give(ok ? S.list[i] : draw_slowly<NT>(x, a.V, R, p, u, &M, S), M);
+  const u64 drawn = ok ? S.list[i] : draw_slowly<NT>(x, a.V, R, p, u, &M, S);  // (sets M: before it is read)
+  give(drawn, M);
 }
 
 constexpr int kMaxSmem = 227 * 1024;

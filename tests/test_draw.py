@@ -537,3 +537,19 @@ def test_profiled_times_are_the_last_draws(pkg):
             e.last_kernel_ms()
     finally:
         e.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 40, 300])
+def test_probability_of_a_token_among_many_equal_ones(pkg, eng, rows):
+    """More equal logits at a border than are collected: the kept mass is the one
+    that the selection over the whole row finds, not an earlier estimate."""
+    import torch
+    V = 60000
+    x = torch.zeros((rows, V), device="cuda")
+    x[:, ::3] = -1.0
+    x[:, 7] = 2.0
+    P = pkg.draw_params(rows, temperature=1.0, top_p=0.5, min_p=[0.0, 0.2] * (rows // 2), top_k=[0, 9001] * (rows // 2))
+    u = np.random.default_rng(rows).random(rows)
+    ids, probs, _ = eng.draw_batch(x, P, u)
+    check(ids, probs, x, P, u)
