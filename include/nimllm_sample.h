@@ -379,18 +379,24 @@ typedef struct nls_g4_weights {
  *  x  nb rows of cols activations of type xtype, ldx >= cols values apart
  *  y  nb rows of w->rows values of type ytype, ldy >= w->rows apart; what lies
  *     behind a row's w->rows values is left as it was
- * Weights are not rounded on the way. Up to 12 batch rows (4 with groups of
- * 32): activations enter as fixed-point numbers of 31 bits against the largest
- * magnitude of the row's 128 columns around them (each is off by 2^-31 of that
- * magnitude at most), and a group's products are summed exactly, in integers.
- * More rows: the products are exact (fp32 activations are taken as three
+ * Weights are not rounded on the way. The batch rows are taken in passes, one
+ * way or the other: while more than 12 rows are left (4 with groups of 32),
+ * the next 64 (32 with groups of 64 or fp32 activations, 16 with groups of 32)
+ * or what is left of them in floating point; the last 12 (4) or fewer in
+ * integers.
+ *  Integers: activations enter as fixed-point numbers of 31 bits against the
+ * largest magnitude of the row's 128 columns around them (each is off by 2^-31
+ * of that magnitude at most), and a group's products are summed exactly.
+ *  Floating point: the products are exact (fp32 activations are taken as three
  * bfloat16 parts) and are summed in fp32 per group; fp32 and bfloat16
  * activations are shifted by 2^-12 on the way, so that sums before the scales
- * cannot overflow, and what they lose lies below 2^-110. Either way the
- * groups' terms are summed in fp32 and rounded once to ytype; a row's bits
- * depend on nb through the way taken. Scales and minimums are below 2^80 in
- * magnitude (larger ones may overflow inside). A batch row that holds an
- * infinity or a NaN gets non-finite logits; the other rows are unaffected.
+ * cannot overflow, and what they lose lies below 2^-110.
+ * Either way the groups' terms are summed in fp32 and rounded once to ytype. A
+ * row's bits depend on the size of its pass, and so on nb and its place; equal
+ * rows of a pass get equal bits, those that a call with the pass's rows alone
+ * gives. Scales and minimums are below 2^80 in magnitude (larger ones may
+ * overflow inside). A batch row that holds an infinity or a NaN gets non-finite
+ * logits; the other rows are unaffected.
  * The same call gives the same bits every time. A pipeline wait that runs out
  * (nls_set_wait_limit) gives NLS_ERR_TIMEOUT and leaves y undefined.
  * Workspace: the handle's, grown by the first call of a size (make that call

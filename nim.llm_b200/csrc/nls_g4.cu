@@ -118,7 +118,7 @@ __host__ __device__ constexpr int x_half(Op op, int nbt, int regions, int parts)
                        : mma_n(op, nbt) * (parts * kHalf * 2 + regions * 4);
 }
 
-// How a launch of nb batch rows goes.
+// How a launch of nb batch rows goes, `left` of the call's rows being left.
 struct Way {
   Op op;
   int nb, nbt, n, parts;

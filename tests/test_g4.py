@@ -486,3 +486,30 @@ def test_a_wait_that_runs_out_is_an_error(pkg, eng, rows, cols, nb):
             eng.set_wait_limit(200 * 1000 * 1000)
         assert e.value.status == pkg._abi.NLS_ERR_TIMEOUT
         assert torch.equal(eng.g4_matmul(w, x), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", DTYPES)
+@pytest.mark.parametrize("group,mins", [(32, True), (64, False), (128, True)])
+def test_bits_of_a_pass(pkg, eng, xt, group, mins):
+    """Batch rows are taken in passes; a pass gives its rows the bits of a call
+    of its own, and equal rows of a pass, wherever they stand in it, equal bits."""
+    import torch
+    per = 64 // max(1, 128 // group)
+    if xt == "f32":
+        per = min(per, 32)
+    few = 4 if group == 32 else 12
+    w = make(pkg, 5003, 1184, group, "f16", mins, seed=7)
+    g = torch.Generator().manual_seed(7)
+    for nb in (few, few + 1, per, per + few, per + few + 1, 2 * per + 3, 5 * per + 1):
+        x = torch.randn((nb, 1184), generator=g).to(_dt(xt)).cuda()
+        y = eng.g4_matmul(w, x, out_dtype=torch.float32)
+        at = 0
+        while at < nb:
+            n = min(per, nb - at)
+            if nb - at <= few:
+                n = nb - at
+            assert torch.equal(y[at:at + n], eng.g4_matmul(w, x[at:at + n], out_dtype=torch.float32)), (nb, at)
+            turn = torch.arange(n).roll(n // 2 + 1)
+            assert torch.equal(y[at:at + n][turn], eng.g4_matmul(w, x[at:at + n][turn], out_dtype=torch.float32))
+            at += n
