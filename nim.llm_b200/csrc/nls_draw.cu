@@ -593,8 +593,9 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
   };
   // A token's bin: its distance below `ref` in 1023rds of the span, rounded to a
-  // whole number by adding 2^23 (logits below max - 32 T have no mass; those
-  // below the span are in the last bin). The span is finite and not negative,
+  // whole number by adding 2^23 (those below the span are in the last bin; the
+  // span reaches at least to the smallest of the first logits or to max - 32.5 T,
+  // below which nothing has a mass). The span is finite and not negative,
   // whatever the temperature, and where the first logits seen are all -inf (low
   // is +inf then).
   float ref = 0.0f, span = 0.0f, scale = 0.0f, floor = 0.0f, c1 = 0.0f, c2 = 0.0f;
@@ -604,7 +605,8 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   // from, to: the span; seen: the largest logit so far (what has no mass beside it
   // has none beside a larger one)
   auto set_bins = [&](float from, float to, float seen) {
-    const float widest = fminf((float)(32.5 * p.temperature), 3.402823466e38f);
+    const float above = fmaxf(from - seen, 0.0f);
+    const float widest = fminf((float)(32.5 * p.temperature) + above, 3.402823466e38f);
     ref = from;
     span = to <= from ? fminf(from - to, widest) : widest;
     scale = span > 1e-30f ? (float)(kBins - 1) / span : 0.0f;
@@ -1169,8 +1171,13 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   double total_est = S.est[kBins - 1];
   bool known = false;     // total is exact
   if (by_k) {
+    // All tokens with a mass are kept where there are fewer than top_k, or the
+    // border lies in a bin from e^-32.2 on (e^-31.9 is half a unit): the last bin
+    // of a wide span can hold more tokens than can be collected. (256 x 128256 fp32
+    // at a temperature of 0.1, top-k 400: 131 us, and 1240 with those rows taken by
+    // the selection over the row.)
     const int b = first_bin<NT>(S.tcnt, (double)p.top_k, S);
-    if (b >= 0) {  // (else all tokens with a mass are kept)
+    if (b >= 0 && step * ((double)b - 0.5) + zero > -32.2) {
       ok = look(b, b, kBins, kBins - 1);
       if (ok) {
         const int i = (int)(p.top_k - 1) - (b > 0 ? (int)S.tcnt[b - 1] : 0);

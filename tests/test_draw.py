@@ -553,3 +553,43 @@ def test_probability_of_a_token_among_many_equal_ones(pkg, eng, rows):
     u = np.random.default_rng(rows).random(rows)
     ids, probs, _ = eng.draw_batch(x, P, u)
     check(ids, probs, x, P, u)
+
+
+def draw_us(eng, x, P, u):
+    """The least of some calls' device times, L2 flushed before each."""
+    import torch
+    P = torch.from_numpy(P.view(np.uint8).copy()).cuda()
+    u = torch.from_numpy(u).cuda()
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    best = float("inf")
+    for _ in range(6):
+        flush.zero_()
+        a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+        a.record()
+        eng.draw_batch(x, P, u, check=False)
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dt", [(4, "f32"), (64, "bf16"), (256, "f32")])
+@pytest.mark.parametrize("T", [0.05, 0.1, 0.2])
+def test_top_k_beyond_the_tokens_with_mass(pkg, eng, rows, dt, T):
+    """Low temperatures leave fewer tokens with a mass than top-k keeps: all of
+    them are kept, and no row goes to the selection over the whole row."""
+    import torch
+    V = 128256
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn((rows, V), generator=g, device="cuda") * 2.5).to(_dt(dt))
+    u = np.random.default_rng(rows).random(rows)
+    plain = draw_us(eng, x, pkg.draw_params(rows, temperature=T, top_p=0.999), u)
+    for k in (300, 400, 600, 1000, 3000, 5000, 20000):
+        for top_p in (1.0, 0.9):
+            P = pkg.draw_params(rows, temperature=T, top_k=k, top_p=top_p)
+            ids, probs, _ = eng.draw_batch(x, P, u)
+            some = [0, rows // 2, rows - 1]
+            check(ids[some], probs[some], x[some], P[some], u[some])
+            us = draw_us(eng, x, P, u)
+            assert us < 4 * plain, f"top-k {k}: {us} us, without it {plain} us"
