@@ -59,7 +59,7 @@ constexpr int kMaxCluster = 16;
 constexpr int kBins = 1024;
 constexpr int kIdxBits = 18;
 constexpr int kList = 2048;           // tokens the first CTA collects and sorts
-constexpr int kMine = 1024;           // tokens a CTA contributes at most
+constexpr int kMine = 1024;           // tokens a CTA hands over together
 constexpr double kUnit = 35184372088832.0;  // 2^45
 constexpr int kMaxWarps = 32;
 constexpr int kPow2 = 512;            // the exponential's table
@@ -790,26 +790,34 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   const Row R(top, p.temperature, S.pow2);
 
   // Tokens go to the (first) CTA's list (its count passes kList where they do
-  // not all fit): one by one by each thread, then, from the other CTAs' own
-  // lists, all together. The latter ends with a barrier of all.
+  // not all fit): one by one by each thread, then, from the CTAs' own lists, all
+  // together. The latter ends with a barrier of all. What a CTA's own list has no
+  // room for goes to the first CTA's at once: where most of a row is masked, the
+  // tokens of one CTA may be all there are. (64 x 150001 bfloat16 nucleus rows with
+  // the second half masked: 1100 us with those rows left to the selection over
+  // the row, 80 so.)
   auto put = [&](float v, int i) {
     const unsigned at = atomicAdd(STREAM ? &S.n_list : &S.n_mine, 1u);
     if (STREAM) {
       if (at < kList) S.list[at] = Row::comp(v, i);
-    } else {
-      if (at < kMine) S.mine[at] = Row::comp(v, i);
+    } else if (at < kMine) {
+      S.mine[at] = Row::comp(v, i);
+    } else if (at < kList) {
+      Shared& D = remote(0);
+      const unsigned there = atomicAdd(&D.n_list, 1u);
+      if (there < kList) D.list[there] = Row::comp(v, i);
     }
   };
   auto hand_over = [&] {
     __syncthreads();
     if constexpr (!STREAM) {
-      const unsigned n = S.n_mine;
+      const unsigned n = min(S.n_mine, (unsigned)kMine);
       Shared& D = remote(0);
-      if (tid == 0) S.value = atomicAdd(&D.n_list, n <= kMine ? n : (unsigned)kList + 1u);
+      if (tid == 0) S.value = atomicAdd(&D.n_list, S.n_mine <= kList ? n : (unsigned)kList + 1u);
       __syncthreads();
       if (tid == 0) S.n_mine = 0;
       const unsigned at = (unsigned)S.value;
-      if (n <= kMine && at + n <= kList)
+      if (at + n <= kList)
         for (unsigned i = tid; i < n; i += NT) D.list[at + i] = S.mine[i];
       cluster.sync();
     }

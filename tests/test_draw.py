@@ -593,3 +593,24 @@ def test_top_k_beyond_the_tokens_with_mass(pkg, eng, rows, dt, T):
             check(ids[some], probs[some], x[some], P[some], u[some])
             us = draw_us(eng, x, P, u)
             assert us < 4 * plain, f"top-k {k}: {us} us, without it {plain} us"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dt,keep", [(64, "bf16", (0, 75000)), (64, "bf16", (0, 120000)), (64, "f16", (75001, 150001)),
+                                          (40, "bf16", (1, 75003)), (16, "f32", (60000, 90000)), (2, "f32", (140000, 150001))])
+def test_a_row_whose_tokens_lie_in_one_part(pkg, eng, rows, dt, keep):
+    """All else masked: the CTA of that part collects all there is to collect,
+    and no row goes to the selection over the whole row."""
+    import torch
+    V = 150001
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, V), generator=g, device="cuda").to(_dt(dt))
+    y = torch.full_like(x, -float("inf"))
+    y[:, keep[0]:keep[1]] = x[:, keep[0]:keep[1]]
+    u = np.random.default_rng(rows).random(rows)
+    for P in (pkg.draw_params(rows, top_p=0.9), pkg.draw_params(rows, top_k=1500, top_p=0.95)):
+        ids, probs, _ = eng.draw_batch(y, P, u)
+        some = np.unique(np.linspace(0, rows - 1, 12).astype(int))
+        check(ids[some], probs[some], y[some], P[some], u[some])
+        plain, us = draw_us(eng, x, P, u), draw_us(eng, y, P, u)
+        assert us < 4 * plain, f"{us} us, without a mask {plain} us"
