@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   const double u = a.uniforms ? a.uniforms[row] : -1.0;
   const bool by_k = p.top_k > 0 && p.top_k < a.V, by_p = p.top_p > 0.0 && p.top_p < 1.0, by_m = p.min_p > 0.0;
   const bool greedy = kind_of(p) == 0, few = kind_of(p) == 1;
+  const bool masses = !greedy && !few;
 
   // The row, or the CTA's slice: vectors [v0, v0 + nv), counted from the 16-byte
   // boundary at or before the first logit. Vectors that reach past the row's
@@ -534,7 +535,29 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     }
   };
 
-  float top = -INFINITY, low = INFINITY, cut = -INFINITY;
+  // The largest logit, and (for masses) the smallest of the first ones that have a
+  // mass beside it: what is masked, by -inf or by a finite value, is not in the
+  // span of the bins. (-1e9 on one logit made that span 32.5 T, its bins too full to collect,
+  // and 64 x 151936 bfloat16 nucleus rows 1700 us instead of 80.)
+  float top = -INFINITY, low = -INFINITY, cut = -INFINITY;
+  const float depth = fminf((float)(36.0 * p.temperature), 3.402823466e38f);
+  // the low of a part of the row whose largest logit is t, beside the largest of
+  // more of it
+  auto low_beside = [&](float t, float l, float largest) {
+    const float f = largest - depth;
+    return t >= f && t > -INFINITY ? fmaxf(l, f) : INFINITY;
+  };
+  // top and low of n parts, a lane each (the same in every lane afterwards)
+  auto join = [&](const float* t, const float* l, int n) {
+    const float mine = lane < n ? t[lane] : -INFINITY;
+    top = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!masses) return;
+    low = low_beside(mine, lane < n ? l[lane] : INFINITY, top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  };
   int best = 0;  // the first vector that holds this thread's largest logit
   // A cut that at least k of the block's values v (one per thread) reach, and
   // not many more: every warp's j-th largest, j = ceil(k / warps) (descending
@@ -596,7 +619,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   // whole number by adding 2^23 (those below the span are in the last bin; the
   // span reaches at least to the smallest of the first logits or to max - 32.5 T,
   // below which nothing has a mass). The span is finite and not negative,
-  // whatever the temperature, and where the first logits seen are all -inf (low
+  // whatever the temperature, and where the first logits seen are all -inf (`to`
   // is +inf then).
   float ref = 0.0f, span = 0.0f, scale = 0.0f, floor = 0.0f, c1 = 0.0f, c2 = 0.0f;
   constexpr float kWhole = 8388608.0f;  // 2^23
@@ -635,7 +658,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   // A streamed row's first pass fills the bins too, from the largest of its first
   // logits and a quarter of their span above; a larger one makes a pass of its
   // own necessary.
-  const bool binned = STREAM && !greedy && !few && p.temperature > 0.0;
+  const bool binned = STREAM && masses && p.temperature > 0.0;
   {
     constexpr int U = 4;
     uint4 q[U], nx[U];
@@ -655,33 +678,39 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
         if (STREAM && vm[t] > top) best = i;
         top = max_nan(top, vm[t]);
       }
-      if (batch == 0) {  // (the span of the bins need not be the whole row's)
+      // (the span of the bins need not be the whole row's: a thread looks at its
+      // first logits, and again where all so far have no mass beside a new one)
+      if (masses && !(low >= top - depth)) {
+        const float f = top - depth;
+        low = INFINITY;
 #pragma unroll
         for (int t = 0; t < U; ++t) {
           const Vec<T> e(q[t]);
 #pragma unroll
-          for (int k = 0; k < VN; ++k) low = fminf(low, e.v[k] == -INFINITY ? INFINITY : e.v[k]);
+          for (int k = 0; k < VN; ++k) low = fminf(low, e.v[k] >= f ? e.v[k] : INFINITY);
         }
       }
       if (STREAM && binned) {
         if (batch == 0) {
-          float m = top, l = low;
+          float m = top;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
-          }
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          float l = low_beside(top, low, m);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
           if (lane == 0) {
             S.fred[0][warp] = m;
             S.fred[1][warp] = l;
           }
           for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;
           __syncthreads();
+          const float mw = lane < kWarps ? S.fred[0][lane] : -INFINITY;
+          m = mw;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            m = fmaxf(m, S.fred[0][w]);
-            l = fminf(l, S.fred[1][w]);
-          }
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          l = low_beside(mw, lane < kWarps ? S.fred[1][lane] : INFINITY, m);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
           m = fmaxf(m, -3.402823466e38f);
           set_bins(fminf(m + 0.25f * fminf(m - fminf(l, m), (float)(32.5 * p.temperature)), 3.402823466e38f), l, m);
         }
@@ -712,9 +741,11 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   if (!STREAM && few) find_cut();
   const float mine_top = top;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (masses) {
+    low = low_beside(mine_top, low, top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
   __syncthreads();
   if (lane == 0) {
@@ -722,11 +753,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
     S.fred[1][warp] = low;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    top = max_nan(top, S.fred[0][w]);
-    low = fminf(low, S.fred[1][w]);
-  }
+  join(S.fred[0], S.fred[1], kWarps);
   if constexpr (!STREAM) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has begun
     if (tid < C) {
@@ -735,10 +762,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       D.low[rank] = low;
     }
     cluster.sync();
-    for (int r = 0; r < C; ++r) {
-      top = max_nan(top, S.top[r]);
-      low = fminf(low, S.low[r]);
-    }
+    join(S.top, S.low, C);
   }
 
   int err = NLS_OK;
@@ -940,6 +964,26 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 
   // ---- masses of the whole row ------------------------------------------------
   __syncthreads();
+  if (few) {  // (its first pass took no low)
+    const float f = top - depth;
+    low = INFINITY;
+    vectors([&](int, const uint4& q) {
+      if (!(vec_max<T>(q) >= f)) return;
+      const Vec<T> e(q);
+#pragma unroll
+      for (int k = 0; k < VN; ++k) low = fminf(low, e.v[k] >= f ? e.v[k] : INFINITY);
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    if (lane == 0) S.fred[0][warp] = low;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) low = fminf(low, S.fred[0][w]);
+    if constexpr (!STREAM) {
+      if (tid < C) remote(tid).low[rank] = low;
+      cluster.sync();
+      for (int r = 0; r < C; ++r) low = fminf(low, S.low[r]);
+    }
+  }
   if (!binned || !(top <= ref)) {
     set_bins(top, low, top);
     for (int i = tid; i < kBins; i += NT) S.bins[0][i] = S.bins[1][i] = 0;

@@ -614,3 +614,30 @@ def test_a_row_whose_tokens_lie_in_one_part(pkg, eng, rows, dt, keep):
         check(ids[some], probs[some], y[some], P[some], u[some])
         plain, us = draw_us(eng, x, P, u), draw_us(eng, y, P, u)
         assert us < 4 * plain, f"{us} us, without a mask {plain} us"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dt", [(4, "f32"), (64, "bf16"), (64, "f16"), (200, "f32")])
+@pytest.mark.parametrize("std,given", [(1.0, dict(top_p=0.9)), (2.5, dict(temperature=2.0, top_p=0.95)),
+                                       (1.0, dict(temperature=1.5, min_p=0.01))])
+def test_masked_logits_do_not_slow_a_row_down(pkg, eng, rows, dt, std, given):
+    """Logits masked by a finite value or by -inf, a few or many, anywhere in the
+    row: the same tokens as the definition's, and no row goes to the selection
+    over the whole row, which takes twenty times as long."""
+    import torch
+    V = 150001
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn((rows, V), generator=g, device="cuda") * std).to(_dt(dt))
+    rng = np.random.default_rng(rows)
+    P, u = pkg.draw_params(rows, **given), rng.random(rows)
+    plain = draw_us(eng, x, P, u)
+    low = float(torch.finfo(_dt(dt)).min)
+    for what in (slice(0, 1), slice(77, 78), slice(0, 40000), slice(0, 140000), slice(120000, V), slice(0, V, 2)):
+        for value in (low, -float("inf"), -3e4):
+            y = x.clone()
+            y[:, what] = value
+            ids, probs, _ = eng.draw_batch(y, P, u)
+            some = [0, rows // 2, rows - 1]
+            check(ids[some], probs[some], y[some], P[some], u[some])
+            us = draw_us(eng, y, P, u)
+            assert us < 4 * plain, f"{what} {value}: {us} us, without a mask {plain} us"
