@@ -1260,14 +1260,18 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
       m1 = fmin(m1, S.est[q1] * wide);
     }
     if (by_m) {
-      // the bin where min_p lies
+      // the bin where min_p lies (two, next to a border: bin() is in fp32), and the
+      // mass down to there; the first token is always kept
       const double lb = step < 0.0 ? fmax(0.0, fmin((log(p.min_p) - zero) / step, (double)kBins)) : (double)kBins;
-      const int b = min(kBins - 1, (int)lb);
-      m = fmin(m, S.est[b]);
-      m1 = fmin(m1, S.est[min(kBins - 1, b + 1)] * wide);
-      m0 = fmin(m0, b >= 2 ? S.est[b - 2] / wide : 1.0);
+      const int b = min(kBins - 1, (int)(lb + 0.49)), c = min(kBins - 1, (int)(lb + 0.51));
+      const double before = b > 0 ? S.est[b - 1] : 0.0;
+      m = fmin(m, fmax(1.0, before + (lb + 0.5 - (double)b) * (S.est[b] - before)));
+      m1 = fmin(m1, S.est[c] * wide);
+      m0 = fmin(m0, fmax(1.0, before / wide));
     }
-    window(u * m0, u * m, u * m1, kList / 2 - 64, &r0, &r1);
+    // (min-p alone leaves a bin's mass open, and the whole list to the bins that
+    // may hold the token)
+    window(u * m0, u * m, u * m1, by_m && !by_p ? kList - 64 : kList / 2 - 64, &r0, &r1);
     if (q0 <= q1 && r1 + 1 >= q0) {  // one range
       r0 = min(r0, q0);
       r1 = max(r1, q1);

@@ -641,3 +641,24 @@ def test_masked_logits_do_not_slow_a_row_down(pkg, eng, rows, dt, std, given):
             check(ids[some], probs[some], y[some], P[some], u[some])
             us = draw_us(eng, y, P, u)
             assert us < 4 * plain, f"{what} {value}: {us} us, without a mask {plain} us"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,V,dt", [(256, 128256, "f32"), (64, 151936, "bf16"), (8, 262144, "f16")])
+@pytest.mark.parametrize("T,min_p", [(1.0, 0.02), (1.2, 0.05), (1.0, 0.1)])
+def test_min_p_that_keeps_many_tokens(pkg, eng, rows, V, dt, T, min_p):
+    """The border of min-p in a crowded bin: no row goes to the selection over
+    the whole row."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, V), generator=g, device="cuda").to(_dt(dt))
+    rng = np.random.default_rng(rows)
+    plain = draw_us(eng, x, pkg.draw_params(rows, temperature=T), rng.random(rows))
+    P = pkg.draw_params(rows, temperature=T, min_p=min_p)
+    for _ in range(4):
+        u = rng.random(rows)
+        ids, probs, _ = eng.draw_batch(x, P, u)
+        some = np.unique(np.linspace(0, rows - 1, 12).astype(int))
+        check(ids[some], probs[some], x[some], P[some], u[some])
+        us = draw_us(eng, x, P, u)
+        assert us < 4 * plain, f"{us} us, without min-p {plain} us"
