@@ -122,9 +122,9 @@ struct Row {
   const double* pow2;
   __device__ __forceinline__ Row(float mx, double T, const double* table) : top((double)mx), pow2(table) {
     scale = __dmul_rn(fmin(1.0 / T, 1e300), 738.65986093514925);
-    // e^-36 is less than half a unit (the float nearest to max - 36 T is not
-    // above any that e^-32 lies above)
-    floor = fmaxf((float)__dsub_rn(top, __dmul_rn(36.0, T)), -3.402823466e38f);
+    // e^-32.2 is less than half a unit (0.37 of one), and a logit below the float
+    // nearest to max - 32.2 T lies below that itself
+    floor = fmaxf((float)__dsub_rn(top, __dmul_rn(32.2, T)), -3.402823466e38f);
   }
   static __device__ __forceinline__ u64 comp(float v, int i) { return ((u64)(~fkey(v)) << kIdxBits) | (u64)i; }
   static __device__ __forceinline__ float value(u64 c) { return fkey_inv(~(uint32_t)(c >> kIdxBits)); }
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   // span of the bins. (-1e9 on one logit made that span 32.5 T, its bins too full to collect,
   // and 64 x 151936 bfloat16 nucleus rows 1700 us instead of 80.)
   float top = -INFINITY, low = -INFINITY, cut = -INFINITY;
-  const float depth = fminf((float)(36.0 * p.temperature), 3.402823466e38f);
+  const float depth = fminf((float)(32.2 * p.temperature), 3.402823466e38f);
   // the low of a part of the row whose largest logit is t, beside the largest of
   // more of it
   auto low_beside = [&](float t, float l, float largest) {
@@ -1223,21 +1223,19 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
   double total_est = S.est[kBins - 1];
   bool known = false;     // total is exact
   if (by_k) {
-    // All tokens with a mass are kept where there are fewer than top_k, or the
-    // border lies in a bin from e^-32.2 on (e^-31.9 is half a unit): the last bin
-    // of a wide span can hold more tokens than can be collected. (256 x 128256 fp32
-    // at a temperature of 0.1, top-k 400: 131 us, and 1240 with those rows taken by
-    // the selection over the row.)
+    // (no bin: all tokens with a mass are kept)
     const int b = first_bin<NT>(S.tcnt, (double)p.top_k, S);
-    if (b >= 0 && step * ((double)b - 0.5) + zero > -32.2) {
+    if (b >= 0) {
       ok = look(b, b, kBins, kBins - 1);
       if (ok) {
+        // (past the bin's tokens: they are all kept as well, the border lies among
+        // tokens without a mass, which the bins of a first pass may count)
         const int i = (int)(p.top_k - 1) - (b > 0 ? (int)S.tcnt[b - 1] : 0);
-        ok = i < n;
         __syncthreads();
+        if (i >= n && tid == 0) S.value = z.all;
 #pragma unroll
         for (int k = 0; k < kPerList; ++k)
-          if (i == place(k)) S.value = run[k];
+          if (i == place(k) && i < n) S.value = run[k];
         __syncthreads();
         total = S.value;
         total_est = (double)total / kUnit;
