@@ -380,10 +380,10 @@ typedef struct nls_g4_weights {
  *  y  nb rows of w->rows values of type ytype, ldy >= w->rows apart; what lies
  *     behind a row's w->rows values is left as it was
  * Weights are not rounded on the way. The batch rows are taken in passes, one
- * way or the other: while more than 12 rows are left (4 with groups of 32),
- * the next 64 (32 with groups of 64 or fp32 activations, 16 with groups of 32)
- * or what is left of them in floating point; the last 12 (4) or fewer in
- * integers.
+ * way or the other: while more than 12 rows are left (4 with groups of 32, and
+ * with groups of 64 unless activations are fp32), the next 64 (32 with groups
+ * of 64 or fp32 activations, 16 with groups of 32) or what is left of them in
+ * floating point; the last 12 (4) or fewer in integers.
  *  Integers: activations enter as fixed-point numbers of 31 bits against the
  * largest magnitude of the row's 128 columns around them (each is off by 2^-31
  * of that magnitude at most), and a group's products are summed exactly.

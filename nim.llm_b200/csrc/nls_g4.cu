@@ -86,8 +86,8 @@ __host__ __device__ constexpr int acc_cols(Op op) { return (int)kTmemCols - 4 * 
 // The split of a CTA's warps, 24 for unpacking and adding at most (72 registers
 // a thread). Unpacking bytes is cheap, and adding four sums per batch row is
 // not: 8 and 16 (one batch row leaves nothing for a second set). Unpacking to
-// 16 bits is the larger part up to 16 batch rows (88 us with 16 and 8, 100 with
-// 8 and 16, on 128256 x 4096); above, adding is (32 rows: 104 and 100 us).
+// 16 bits is the larger part up to 16 batch rows (81 us with 16 and 8, 87 with
+// 8 and 16, on 128256 x 4096); above, adding is (32 rows: 95.5 and 94 us).
 __host__ __device__ constexpr int unpack_warps(Op op, int nbt) { return op != Op::kI8 && nbt <= 16 ? 16 : 8; }
 __host__ __device__ constexpr int add_warps(Op op, int nbt) {
   return op != Op::kI8 ? (nbt <= 16 ? 8 : 16) : nbt == 1 ? 8 : 16;
@@ -104,12 +104,14 @@ __host__ __device__ constexpr int batch_of(Op op, int nb) {
 __host__ __device__ constexpr int mma_n(Op op, int nbt) {
   return op == Op::kI8 ? (nbt <= 4 ? 16 : 4 * nbt) : (nbt <= 16 ? 16 : nbt);
 }
-// The most batch rows the integer way takes. Two buffers of accumulators have
-// to fit in tensor memory (96 columns per tile half and buffer): 4 rows with
-// groups of 32, 12 with groups of 64. With wider ones 12 too, by the times: 12 /
-// 16 rows take 82 / 112 us this way and 84 / 88 us in floating point (128256 x
-// 4096).
-__host__ __device__ constexpr int i8_rows(int regions) { return regions == 4 ? 4 : 12; }
+// The most batch rows the integer way takes. By tensor memory, two buffers of
+// accumulators have to fit (96 columns per tile half and buffer): 4 rows with
+// groups of 32, 12 with groups of 64. By the times, in integers and in floating
+// point: wide groups, 128256 x 4096, 12 rows 76 and 81 us, 16 rows 106 and 81;
+// groups of 64, 151936 x 4096, fp32 activations 5 to 8 rows 117 and 146 us, 9 to
+// 12 138 and 149; 16-bit ones 117 and 92, 138 and 99 (1 to 4 rows in integers: 68
+// to 85).
+__host__ __device__ constexpr int i8_rows(int regions, bool f32) { return regions == 4 || (regions == 2 && !f32) ? 4 : 12; }
 // bytes of a half step's laid-out activations: bytes (and per region and batch
 // row four words for the joining), or 16-bit parts (and per region and column
 // their sum)
@@ -127,7 +129,7 @@ struct Way {
 Way way_of(const G4Args& a, int left) {
   Way w;
   const int regions = regions_of(a.group);
-  w.op = left <= i8_rows(regions) ? Op::kI8 : a.xtype == NLS_DT_F16 ? Op::kF16 : Op::kBF16;
+  w.op = left <= i8_rows(regions, a.xtype == NLS_DT_F32) ? Op::kI8 : a.xtype == NLS_DT_F16 ? Op::kF16 : Op::kBF16;
   w.parts = w.op != Op::kI8 && a.xtype == NLS_DT_F32 ? 3 : 1;
   // regions x N columns: 64 per tile half and buffer. (fp32's three parts: a
   // stage of 64 rows would leave room for one stage only)
@@ -1001,13 +1003,13 @@ const void* kernel_of(int nbt) {
       case 2: return (const void*)g4_kernel<OP, 2, R>;
       case 4: return (const void*)g4_kernel<OP, 4, R>;
     }
-    if constexpr (i8_rows(R) >= 12) {
+    if constexpr (i8_rows(R, true) >= 12) {
       if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
       if (nbt == 12) return (const void*)g4_kernel<OP, 12, R>;
     }
   } else {
     // (fewer rows than these are the integer way's)
-    if constexpr (i8_rows(R) < 8) {
+    if constexpr (i8_rows(R, false) < 8) {
       if (nbt == 8) return (const void*)g4_kernel<OP, 8, R>;
     }
     if (nbt == 16) return (const void*)g4_kernel<OP, 16, R>;

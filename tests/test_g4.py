@@ -498,10 +498,10 @@ def test_bits_of_a_pass(pkg, eng, xt, group, mins):
     per = 64 // max(1, 128 // group)
     if xt == "f32":
         per = min(per, 32)
-    few = 4 if group == 32 else 12
+    few = 4 if group == 32 or (group == 64 and xt != "f32") else 12
     w = make(pkg, 5003, 1184, group, "f16", mins, seed=7)
     g = torch.Generator().manual_seed(7)
-    for nb in (few, few + 1, per, per + few, per + few + 1, 2 * per + 3, 5 * per + 1):
+    for nb in (few, few + 1, 9, per, per + few, per + few + 1, 2 * per + 3, 5 * per + 1):
         x = torch.randn((nb, 1184), generator=g).to(_dt(xt)).cuda()
         y = eng.g4_matmul(w, x, out_dtype=torch.float32)
         at = 0
@@ -513,3 +513,21 @@ def test_bits_of_a_pass(pkg, eng, xt, group, mins):
             turn = torch.arange(n).roll(n // 2 + 1)
             assert torch.equal(y[at:at + n][turn], eng.g4_matmul(w, x[at:at + n][turn], out_dtype=torch.float32))
             at += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("xt", DTYPES)
+def test_groups_of_64_on_both_sides_of_their_ways(pkg, eng, xt, mins):
+    """Groups of 64 leave the integer way after 4 batch rows of 16-bit
+    activations and after 12 of fp32 ones."""
+    import torch
+    w = make(pkg, 2065, 1120, 64, "bf16", mins, seed=12)
+    x = torch.randn((13, 1120), generator=torch.Generator().manual_seed(12)).to(_dt(xt)).cuda()
+    y = [eng.g4_matmul(w, x[:nb], out_dtype=torch.float32) for nb in range(1, 14)]
+    for nb in range(1, 14):
+        check(w, x[:nb], y[nb - 1], f"{nb} rows")
+    last = 12 if xt == "f32" else 4
+    for nb in range(1, last):                              # one way: the same bits
+        assert torch.equal(y[nb - 1][0], y[last - 1][0])
+    assert not torch.equal(y[last - 1], y[last][:last])
