@@ -662,3 +662,23 @@ def test_min_p_that_keeps_many_tokens(pkg, eng, rows, V, dt, T, min_p):
         check(ids[some], probs[some], x[some], P[some], u[some])
         us = draw_us(eng, x, P, u)
         assert us < 4 * plain, f"{us} us, without min-p {plain} us"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dt", [(1, "f32"), (64, "bf16"), (300, "f16")])
+def test_a_row_of_equal_logits_takes_a_bounded_time(pkg, eng, rows, dt):
+    """The selection over the whole row: some twenty passes over it by one CTA, so
+    that a hundred times as long as a row that is read twice is a wide bound; with
+    the additions of equal logits one after the other it was seven hundred."""
+    import torch
+    V = 150001
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn((rows, V), generator=g, device="cuda") * 2.5).to(_dt(dt))
+    y = torch.full_like(x, 0.75)
+    u = np.random.default_rng(rows).random(rows)
+    P = pkg.draw_params(rows, top_p=0.9, min_p=[0.0, 0.3][rows % 2], top_k=70000)
+    ids, probs, _ = eng.draw_batch(y, P, u)
+    some = np.unique(np.linspace(0, rows - 1, 6).astype(int))
+    check(ids[some], probs[some], y[some], P[some], u[some])
+    plain, us = draw_us(eng, x, P, u), draw_us(eng, y, P, u)
+    assert us < 100 * plain, f"{us} us, other rows {plain} us"
