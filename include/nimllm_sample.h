@@ -429,6 +429,14 @@ typedef struct nls_draw_params {
  * taken as real numbers (the masses in fixed point, 2^-45 of the largest,
  * summed exactly) instead of the reference's sequential fp32 sums, and ties at
  * the top-k border going to the lowest index.
+ * The time depends on the settings (a top-k of a hundred or so, or min-p that
+ * keeps few tokens, takes little more than reading the logits; what needs the
+ * mass of the whole row two to four times that), hardly on the logits. A row
+ * with about a thousand or more equal logits at the border of what is kept or
+ * about the drawn token, and about one row in ten thousand of those that need
+ * the whole row's mass, takes some twenty passes over its logits: 1.5 to 2 ms
+ * for 150000 of them, up to 35 ms where nearly all have one of two or three
+ * values.
  *  logits    rows of vocab values of type ltype, ld >= vocab values apart,
  *            aligned to their type
  *  params    [rows]
@@ -459,8 +467,8 @@ NLS_API nls_status nls_g4_lm_head_draw(nls_handle* h, const nls_g4_weights* w, c
 /* Per-kernel timing of later calls on this handle (tracing; no counterpart
  * in the reference, which only times whole generations with epochTime,
  * chat.nim:191,246-247). With `on` set, every sampling call (draws included)
- * records CUDA events around each of its kernels on the call's stream; the
- * projections are not timed, in calls that do both neither. */
+ * records CUDA events around each of its kernels on the call's stream. The
+ * projections are not timed, nor is that part of a call that does both. */
 NLS_API nls_status nls_set_profiling(nls_handle* h, int32_t on);
 
 /* Device times in milliseconds of the last profiled call, each measured from

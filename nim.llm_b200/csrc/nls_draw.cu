@@ -15,8 +15,8 @@
 // Where a row runs: with many rows, one CTA per row (four to an SM), which
 // streams the row from memory; with few, a thread-block cluster per row, each
 // CTA with its slice of the row in shared memory. Then one of two ways:
-//  * Few candidates (top-k up to 32 per warp; min-p alone): a cut that at least
-//    the needed tokens reach -- for top-k a quantile of the threads' maxima,
+//  * Few candidates (top-k up to half the CTA's threads; min-p alone): a cut that at
+//    least the needed tokens reach -- for top-k a quantile of the threads' maxima,
 //    since the k-th largest of some of the logits is no larger than the k-th
 //    largest of all -- and the tokens above it, collected and sorted by the
 //    (first) CTA. A streamed row takes the cut from its first logits and reads
@@ -28,15 +28,17 @@
 //    the tokens there, which are sorted. (A token adds its mass relative to its
 //    bin's middle, by a polynomial of degree two in fp32, with one atomic.
 //    Binning the exact masses instead took 35 more instructions per logit and
-//    two returning atomics.) What the sums do not confirm, and bins that hold
-//    too many tokens (very many equal logits), goes to a radix selection over
-//    comp, ten bits at a time, by the (first) CTA.
+//    two returning atomics.) What the sums do not confirm, and bins at a border
+//    that hold too many tokens (from about a thousand equal logits on), goes to a
+//    radix selection over comp, ten bits at a time, by the (first) CTA: 1.5 to 2
+//    ms a row of 150000 logits, and up to 35 ms where nearly all of them have one
+//    of two or three values, whose additions meet at one address.
 // What bounds it: reading the logits for the first way; for the second the
 // instructions of the masses (about 40 per logit, 11 of them fp64, in the exact
 // pass); for a few rows the chain of barriers of one row. Measured: 256 x 128256
-// fp32, highest logit 29 us (4.5 TB/s), top-k 50 43 us, nucleus 157 us, settings
-// of every kind 110 us; 2048 x 151936 bfloat16 top-k 50 252 us (2.5 TB/s); 64 x
-// 151936 bfloat16 nucleus 72 us; one row of 128256: top-k with top-p and min-p
+// fp32, highest logit 29 us (4.5 TB/s), top-k 50 42 us, nucleus 161 us, settings
+// of every kind 112 us; 2048 x 151936 bfloat16 top-k 50 248 us (2.5 TB/s); 64 x
+// 151936 bfloat16 nucleus 75 us; one row of 128256: top-k with top-p and min-p
 // 19 us, nucleus 36 us.
 #include <cooperative_groups.h>
 
@@ -1350,9 +1352,12 @@ cudaError_t launch_draw(const DrawArgs& a, int sm_count, cudaStream_t st) {
     C = std::max({C, need, 1});
     if ((int64_t)C * a.rows > sm_count && nvec > 128) {
       // 1024 threads to an SM: four rows, or two where there are not that many
-      // (256 x 128256 fp32 with 512 and with 1024 threads a row: top-k 43 and 55
-      // us, nucleus 160 and 169, settings of every kind 111 and 98; 2048 x 151936
-      // bfloat16 top-k with 256 and with 512 threads: 253 and 270 us)
+      // (256 x 128256 fp32 with 512 and with 1024 threads a row: top-k 42 and 53
+      // us, nucleus 162 and 175, settings of every kind 113 and 99; 2048 x 151936
+      // bfloat16 top-k with 256 and with 512 threads: 247 and 266 us, 500 x 50257
+      // fp16 nucleus 149 and 158, 500 x 128256 fp32 of every kind 232 and 153: more
+      // threads are better for the few rows that need masses, and which those are
+      // is not known here)
       const bool many = a.rows > 3 * sm_count;
       auto stream = [&](auto kernel, int threads, std::atomic<int>* set) {
         cudaError_t f = ensure_smem_attr(reinterpret_cast<const void*>(kernel), (int)smem_bytes(0), set);

@@ -33,10 +33,13 @@
 // and 4 packed subtractions per 8 weights, and 4 bytes per packed byte into
 // tensor memory) holds the floating-point way to two thirds of the rate of the
 // integer one at one row. Measured (128256 x 4096, groups of 128, bfloat16: 271
-// MB of weights and scales, 42 us at the rate of a plain copy): 1 / 4 / 12 batch
-// rows 57 / 63 / 80 us (one row 4.7 TB/s), 16 / 32 / 64 rows 84 / 97 / 125 us.
-// About 10 us of each call are outside the stream: two launches, the pipeline's
-// filling and the joining of split tiles.
+// MB of weights and scales, 42 us at the rate of a plain copy; captured calls one
+// after the other): 1 / 4 / 12 batch rows 54 / 59 / 76 us (one row 5.0 TB/s), 16 /
+// 32 / 64 rows 81 / 94 / 122 us. More rows read and unpack the weights again for
+// every 64 of them (128 rows 244 us), with groups of 64 or fp32 activations for
+// every 32, with groups of 32 for every 16 (151936 x 4096: 16 / 32 / 64 rows 138 /
+// 272 / 543 us). About 10 us of each call are outside the stream: two launches,
+// the pipeline's filling and the joining of split tiles.
 //
 // Work: a tile is 256 weight rows (two MMAs of M = 128), a step 256 columns of
 // it: 128 bytes of a row, since the copy of a step costs the copy engine about
