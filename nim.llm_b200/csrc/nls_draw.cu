@@ -553,8 +553,8 @@ __global__ void __launch_bounds__(NT, STREAM ? 1024 / NT : 1) draw_kernel(const 
 
   // The largest logit, and (for masses) the smallest of the first ones that have a
   // mass beside it: what is masked, by -inf or by a finite value, is not in the
-  // span of the bins. (-1e9 on one logit made that span 32.5 T, its bins too full to collect,
-  // and 64 x 151936 bfloat16 nucleus rows 1700 us instead of 80.)
+  // span of the bins. (-1e9 on one logit made that span 32.5 T, its bins too full
+  // to collect, and 64 x 151936 bfloat16 nucleus rows 1700 us instead of 80.)
   float top = -INFINITY, low = -INFINITY, cut = -INFINITY;
   const float depth = fminf((float)(32.2 * p.temperature), 3.402823466e38f);
   // the low of a part of the row whose largest logit is t, beside the largest of
